@@ -227,6 +227,65 @@ int qc_batch_stats(const qc_batch* b, qc_stats* out);
 int qc_batch_ep_handle(qc_batch* b, void* handle, int* device_id);
 int qc_batch_ep_connect(qc_batch* b, const void* handles, const int* device_ids);
 
+/* ---- paged key-value cache (no counterpart in the reference, whose cache is one contiguous block per
+ * layer, model.rs:183-199) ------------------------------------------------------------------------
+ * One layer's cache for several sequences: two pools of pages [n_pages][kvheads][page][head_dim]
+ * (keys, values) of GGML type `kind` (0 F32, 1 F16, 30 BF16) and a table [n_seqs][max_pages] of page
+ * numbers.  Slot j of sequence s is slot j % page of page table[s][j / page].  A cache row (head_dim
+ * values, at most 256) is a multiple of 16 bytes; page may be any number of slots.
+ *
+ * All arguments that are not sizes are DEVICE pointers on one device (pools, q, k, v and out 16-byte
+ * aligned); the call runs on that device and on `stream` (a cudaStream_t of that device; NULL = its
+ * default stream), allocates nothing, keeps nothing between calls and returns once the work is
+ * enqueued, so it can be captured into a CUDA graph.  Errors: qc_last_error().  What lies on the device
+ * is checked there: a row of a sequence >= n_seqs (padding) is skipped and its outputs left as they
+ * were; a length beyond max_pages * page or a page number >= n_pages among the slots a row uses makes
+ * its results NaN (attention), or leaves the slot or the sequence as it was (append, evict).
+ * Calls that write the same cache, weights or outputs must be ordered by the caller. */
+
+/* Row i of k and v ([rows][kvheads][head_dim] f32) goes, rounded to nearest, to slot pos[i] of sequence
+ * seq[i] (seq NULL: sequence i).  The rows of a call have different slots.  weights (may be NULL, as for
+ * qc_paged_attention): the slot's accumulated weights become 0. */
+int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages, uint32_t page, uint32_t kvheads,
+                    uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages, const float* k,
+                    const float* v, uint32_t rows, const uint32_t* seq, const uint32_t* pos, float* weights, void* stream);
+/* Attention of new tokens (ops.rs:57-98 over a paged cache): row i of q ([rows][heads][head_dim] f32)
+ * attends to slots 0..len[i]-1 of sequence seq[i] (seq NULL: sequence i); head h reads KV head
+ * h / (heads / kvheads), at most 32 query heads per KV head.  out = softmax(scale q k^T) v in f32
+ * (scale 0: 1 / sqrt(head_dim)); lse (may be NULL, [rows][heads]) receives log sum exp(scale q k^T).
+ * A row of length 0 gives out 0 and lse -inf; so does one whose scores all overflow to -inf.  Slots a row
+ * does not attend to may hold anything; a non-finite value among those it reads makes its results
+ * non-finite.
+ * weights (may be NULL): [n_seqs][kvheads][max_pages * page] f32; the softmax weights that the rows give
+ * slot j, summed over a KV head's query heads, are added to weights[s][kv head][j], rows of one
+ * sequence in call order.  The results do not depend on timing: the same call gives the same bits. */
+int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, uint32_t n_pages, uint32_t page,
+                       uint32_t kvheads, uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages,
+                       const float* q, uint32_t heads, uint32_t rows, const uint32_t* seq, const uint32_t* len, float scale,
+                       float* out, float* lse, float* weights, void* stream);
+/* Eviction by accumulated attention weight: of a sequence of len[s] > keep slots, every KV head keeps the
+ * last `recent` slots and, of the others, the keep - recent with the largest weights (equal weights: the
+ * lower slot; NaN counts as the smallest).  Their rows and weights move, in their order, to slots
+ * 0..keep-1 of the pages dst_table[s] ([n_seqs][max_pages]; NULL: in place) and to weights_out (may be
+ * weights).  kept ([n_seqs][kvheads][keep]) receives the slots' old numbers (0xffffffff behind the last
+ * one), new_len (may be len) min(len, keep).  A sequence within keep keeps all slots (and is copied
+ * where dst_table names other pages).  Pages of dst_table are written by one sequence only, and are
+ * either not read by this call or, in place, the same pages at the same places. */
+int qc_paged_evict(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages, uint32_t page, uint32_t kvheads,
+                   uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages, const uint32_t* dst_table,
+                   const float* weights, float* weights_out, const uint32_t* len, uint32_t* new_len, uint32_t keep,
+                   uint32_t recent, uint32_t* kept, void* stream);
+
+/* ---- log probabilities (the softmax of sampling.rs:45-56 at temperature 1, unfiltered) ------------
+ * Of each of `rows` logits rows (n floats, `stride` floats apart): the log probabilities of n_ids given
+ * ids (ids, logprobs: [rows][n_ids]; an id >= n gives NaN), the entropy in nats (entropy: [rows], may be
+ * NULL) and the `top` (<= 64, <= n) likeliest ids with theirs, the likeliest first, equal logits by the
+ * lower id (top_ids, top_logprobs: [rows][top]).  A logit of -inf has probability 0; a row that holds
+ * NaN or +inf, or only -inf, gives NaN for every log probability and the entropy (NaN logits come last
+ * among the alternatives).  Device pointers, stream and errors as for the paged cache. */
+int qc_logprobs(const float* logits, uint32_t rows, uint32_t n, uint64_t stride, const uint32_t* ids, uint32_t n_ids,
+                uint32_t top, float* logprobs, float* entropy, uint32_t* top_ids, float* top_logprobs, void* stream);
+
 /* model.rs:202-208: clear the KV cache and set the position to 0. */
 int qc_reset(qc_engine* e);
 int qc_position(const qc_engine* e, uint32_t* pos);

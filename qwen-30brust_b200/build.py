@@ -23,7 +23,7 @@ CUDA_LIB = HERE / "libqwen_cuda.so"
 TOOLS_LIB = HERE / "libqwen_tools.so"
 
 CU_SOURCES = ["matvec.cu", "decode.cu", "token.cu", "engine.cu", "noalloc.cu", "sample.cu", "moe.cu", "batch.cu",
-              "qgemm.cu"]
+              "qgemm.cu", "paged.cu", "logprobs.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

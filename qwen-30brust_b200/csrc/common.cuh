@@ -10,7 +10,8 @@
 namespace qc {
 
 // GGML type ids (reference quant.rs:5-11).
-enum Kind : uint32_t { F32 = 0, F16 = 1, Q4_0 = 2, Q8_0 = 8, Q4_K = 12, Q5_K = 13, Q6_K = 14 };
+// BF16 (30, as GGML numbers it) is a type of cache pages only.
+enum Kind : uint32_t { F32 = 0, F16 = 1, Q4_0 = 2, Q8_0 = 8, Q4_K = 12, Q5_K = 13, Q6_K = 14, BF16 = 30 };
 
 // Device layout of one matrix (or of an expert stack).  A row is processed in
 // "units" of 64 consecutive elements.  Rows are stored in groups of 8,

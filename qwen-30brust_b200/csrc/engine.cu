@@ -65,6 +65,7 @@ void prepare_device(int device) {
   QC_CK(qc::sample_prepare());
   QC_CK(qc::batch_prepare(kMaxSmem));
   QC_CK(qc::qgemm_prepare());
+  QC_CK(qc::paged_prepare());
   done[device] = true;
 }
 
@@ -2056,6 +2057,157 @@ int qc_batch_stats(const qc_batch* b, qc_stats* out) {
     out->kv_bytes = (uint64_t)b->n_seqs * b->e->cfg.layers * 2 * b->kv_floats * 4;
     out->weight_bytes = b->e->weight_bytes;
     out->matvecs = ((5ull + 3ull * b->e->cfg.top) * b->e->cfg.layers + 1) * b->stats.tokens;
+  });
+}
+
+// ---- paged key-value cache, log probabilities -------------------------------------------------
+// Device pointers of callers, checked on the host as far as the host can: alignment, device memory,
+// one device.  The call runs on that device, whatever the current one is.
+namespace {
+
+struct DevicePointers {
+  int device = -1, before = -1;
+  ~DevicePointers() {
+    if (before >= 0 && before != device) cudaSetDevice(before);
+  }
+  void add(const void* p, const char* name, uintptr_t align = 4) {
+    if (!p) return;
+    ensure(reinterpret_cast<uintptr_t>(p) % align == 0, std::string(name) + " is not " + std::to_string(align) + "-byte aligned");
+    cudaPointerAttributes at{};
+    QC_CK(cudaPointerGetAttributes(&at, p));
+    ensure(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, std::string(name) + " is not device memory");
+    if (device < 0) device = at.device;
+    ensure(at.device == device, std::string(name) + " lives on another device than the other arguments");
+  }
+  void enter() {
+    QC_CK(cudaGetDevice(&before));
+    if (before != device) QC_CK(cudaSetDevice(device));
+    prepare_device(device);
+  }
+};
+
+// The cache of a paged call, with every check that needs no device.
+qc::PagedKV paged_kv(uint32_t kind, void* k, void* v, uint32_t n_pages, uint32_t page, uint32_t kvheads, uint32_t head_dim,
+                     const uint32_t* table, uint32_t n_seqs, uint32_t max_pages) {
+  ensure(k && v && table, "null argument");
+  ensure(kind == qc::F32 || kind == qc::F16 || kind == qc::BF16, "cache pages are F32, F16 or BF16");
+  ensure(n_pages && page && kvheads && n_seqs && max_pages, "empty cache");
+  const uint32_t per16 = kind == qc::F32 ? 4 : 8;
+  ensure(head_dim >= per16 && head_dim <= 256 && head_dim % per16 == 0,
+         "cache rows must be a multiple of 16 bytes and at most 256 values");
+  ensure((uint64_t)max_pages * page <= 0x7fffffffull, "more than 2^31 - 1 slots in a sequence");
+  ensure(kvheads <= 0x10000 && (uint64_t)n_pages * page <= 0xffffffffull / kvheads, "more than 2^32 - 1 rows in a pool");
+  ensure((uint64_t)n_seqs * kvheads <= 0x7fffffffull, "too many sequences");
+  return qc::PagedKV{kind, k, v, n_pages, page, kvheads, head_dim, table, n_seqs, max_pages};
+}
+
+}  // namespace
+
+int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages, uint32_t page, uint32_t kvheads,
+                    uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages, const float* k,
+                    const float* v, uint32_t rows, const uint32_t* seq, const uint32_t* pos, float* weights, void* stream) {
+  return api(nullptr, [&] {
+    const qc::PagedKV c = paged_kv(kind, k_pages, v_pages, n_pages, page, kvheads, head_dim, table, n_seqs, max_pages);
+    if (!rows) return;
+    ensure(k && v && pos, "null argument");
+    ensure(seq || rows <= n_seqs, "more rows than sequences");
+    ensure(rows <= 0x7fffffffu, "too many rows");
+    DevicePointers at;
+    at.add(k_pages, "k_pages", 16);
+    at.add(v_pages, "v_pages", 16);
+    at.add(table, "table");
+    at.add(k, "k", 16);
+    at.add(v, "v", 16);
+    at.add(seq, "seq");
+    at.add(pos, "pos");
+    at.add(weights, "weights");
+    at.enter();
+    QC_CK(qc::launch_paged_append(c, k, v, rows, seq, pos, weights, static_cast<cudaStream_t>(stream)));
+  });
+}
+
+int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, uint32_t n_pages, uint32_t page,
+                       uint32_t kvheads, uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages,
+                       const float* q, uint32_t heads, uint32_t rows, const uint32_t* seq, const uint32_t* len, float scale,
+                       float* out, float* lse, float* weights, void* stream) {
+  return api(nullptr, [&] {
+    const qc::PagedKV c = paged_kv(kind, const_cast<void*>(k_pages), const_cast<void*>(v_pages), n_pages, page, kvheads,
+                                   head_dim, table, n_seqs, max_pages);
+    ensure(heads && heads % kvheads == 0 && heads / kvheads <= 32,
+           "heads must be a multiple of kvheads, at most 32 query heads per KV head");
+    ensure(std::isfinite(scale), "scale must be finite");
+    if (!rows) return;
+    ensure(q && len && out, "null argument");
+    ensure(seq || rows <= n_seqs, "more rows than sequences");
+    ensure((uint64_t)rows * kvheads <= 0x7ffffffull, "too many rows");
+    DevicePointers at;
+    at.add(k_pages, "k_pages", 16);
+    at.add(v_pages, "v_pages", 16);
+    at.add(table, "table");
+    at.add(q, "q", 16);
+    at.add(seq, "seq");
+    at.add(len, "len");
+    at.add(out, "out", 16);
+    at.add(lse, "lse");
+    at.add(weights, "weights");
+    at.enter();
+    qc::PagedRows r{q, heads, rows, seq, len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale, out, lse, weights};
+    QC_CK(qc::launch_paged_attention(c, r, static_cast<cudaStream_t>(stream)));
+  });
+}
+
+int qc_paged_evict(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages, uint32_t page, uint32_t kvheads,
+                   uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages, const uint32_t* dst_table,
+                   const float* weights, float* weights_out, const uint32_t* len, uint32_t* new_len, uint32_t keep,
+                   uint32_t recent, uint32_t* kept, void* stream) {
+  return api(nullptr, [&] {
+    const qc::PagedKV c = paged_kv(kind, k_pages, v_pages, n_pages, page, kvheads, head_dim, table, n_seqs, max_pages);
+    ensure(weights && weights_out && len && new_len && kept, "null argument");
+    ensure(keep > 0 && keep <= (uint64_t)max_pages * page, "keep must be in 1..=max_pages * page");
+    ensure(recent <= keep, "recent must be at most keep");
+    DevicePointers at;
+    at.add(k_pages, "k_pages", 16);
+    at.add(v_pages, "v_pages", 16);
+    at.add(table, "table");
+    at.add(dst_table, "dst_table");
+    at.add(weights, "weights");
+    at.add(weights_out, "weights_out");
+    at.add(len, "len");
+    at.add(new_len, "new_len");
+    at.add(kept, "kept");
+    at.enter();
+    qc::PagedEvict e{weights, len, keep, recent, dst_table ? dst_table : table, kept, new_len, weights_out};
+    QC_CK(qc::launch_paged_evict(c, e, static_cast<cudaStream_t>(stream)));
+  });
+}
+
+namespace {
+void check_logprobs(uint32_t n, const uint32_t* ids, uint32_t n_ids, uint32_t top, const float* logprobs,
+                    const uint32_t* top_ids, const float* top_logprobs) {
+  ensure(n > 0, "empty logits");
+  ensure(top <= n && top <= qc::kMaxTop, "top must be at most 64 and at most the number of logits");
+  ensure((!n_ids || (ids && logprobs)) && (!top || (top_ids && top_logprobs)), "null argument");
+}
+}  // namespace
+
+int qc_logprobs(const float* logits, uint32_t rows, uint32_t n, uint64_t stride, const uint32_t* ids, uint32_t n_ids,
+                uint32_t top, float* logprobs, float* entropy, uint32_t* top_ids, float* top_logprobs, void* stream) {
+  return api(nullptr, [&] {
+    check_logprobs(n, rows ? ids : nullptr, rows ? n_ids : 0, rows ? top : 0, logprobs, top_ids, top_logprobs);
+    ensure(n <= 0x7fffffffu && rows <= 0x7ffffffu, "too many logits");
+    ensure(stride >= n || rows < 2, "rows overlap: stride is below n");
+    if (!rows) return;
+    ensure(logits, "null argument");
+    DevicePointers at;
+    at.add(logits, "logits");
+    at.add(ids, "ids");
+    at.add(logprobs, "logprobs");
+    at.add(entropy, "entropy");
+    at.add(top_ids, "top_ids");
+    at.add(top_logprobs, "top_logprobs");
+    at.enter();
+    qc::LogprobArgs a{logits, nullptr, rows, n, stride, ids, n_ids, top, logprobs, entropy, top_ids, top_logprobs};
+    QC_CK(qc::launch_logprobs(a, static_cast<cudaStream_t>(stream)));
   });
 }
 

@@ -297,6 +297,56 @@ void launch_batch_qkprep(const BatchArgs& a, uint32_t layer, const float* q_norm
                          const float* k, const float* v, uint32_t T, cudaStream_t s);
 void launch_batch_attention(const BatchArgs& a, uint32_t layer, const float* q, float* out, uint32_t T, cudaStream_t s);
 void launch_batch_finite(const float* v, uint64_t n, uint32_t* flag, cudaStream_t s);
+// ---- paged key-value cache (paged.cu) ----------------------------------------------------------
+// One layer's cache: pools [n_pages][kvheads][page][D] of keys and values in `kind` (F32, F16, BF16)
+// and a table [n_seqs][max_pages] of page numbers.
+struct PagedKV {
+  uint32_t kind;
+  void *k, *v;
+  uint32_t n_pages, page, kvheads, D;
+  const uint32_t* table;
+  uint32_t n_seqs, max_pages;
+};
+// Query rows of one call: row i attends to slots 0..len[i]-1 of sequence seq[i] (seq null: i).
+struct PagedRows {
+  const float* q;  // [rows][heads][D]
+  uint32_t heads, rows;
+  const uint32_t *seq, *len;
+  float scale;
+  float *out, *lse;  // [rows][heads][D], [rows][heads] or null
+  float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights
+};
+constexpr uint32_t kNoSlot = 0xffffffffu;
+struct PagedEvict {
+  const float* weights;
+  const uint32_t* len;        // [n_seqs]
+  uint32_t keep, recent;
+  const uint32_t* dst_table;  // [n_seqs][max_pages]: where the kept rows go (may be the cache's table)
+  uint32_t* kept;             // [n_seqs][kvheads][keep]
+  uint32_t* new_len;          // [n_seqs] (may be len)
+  float* weights_out;         // (may be weights)
+};
+cudaError_t paged_prepare();
+cudaError_t launch_paged_append(const PagedKV& c, const float* k, const float* v, uint32_t rows, const uint32_t* seq,
+                                const uint32_t* pos, float* weights, cudaStream_t st);
+cudaError_t launch_paged_attention(const PagedKV& c, const PagedRows& r, cudaStream_t st);
+cudaError_t launch_paged_evict(const PagedKV& c, const PagedEvict& e, cudaStream_t st);
+
+// ---- log probabilities (logprobs.cu) -----------------------------------------------------------
+struct LogprobArgs {
+  const float* logits;  // rows of n, `stride` floats apart
+  const uint32_t* src;  // row numbers in logits (null: 0, 1, ...)
+  uint32_t rows, n;
+  uint64_t stride;
+  const uint32_t* ids;  // [rows][n_ids]
+  uint32_t n_ids, top;
+  float *logprobs, *entropy;  // [rows][n_ids]; [rows] or null
+  uint32_t* top_ids;          // [rows][top]
+  float* top_logprobs;
+};
+constexpr uint32_t kMaxTop = 64;
+cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st);
+
 // n keystream words of the sampler (advancing it), for reproducibility checks.
 void launch_sampler_words(SamplerDev* s, uint32_t n, uint32_t* out, cudaStream_t st);
 

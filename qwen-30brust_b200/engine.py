@@ -33,6 +33,7 @@ EXPORTS = (
     "qc_engine_sample", "qc_decode_sample", "qc_moe_layer", "qc_batch_create", "qc_batch_destroy",
     "qc_batch_forward", "qc_batch_reset", "qc_batch_position", "qc_batch_logits_device", "qc_batch_sample",
     "qc_batch_decode_sample", "qc_batch_stats", "qc_batch_ep_handle", "qc_batch_ep_connect",
+    "qc_paged_append", "qc_paged_attention", "qc_paged_evict", "qc_logprobs",
 )
 
 
@@ -149,6 +150,11 @@ def lib() -> C.CDLL:
         L.qc_batch_stats.argtypes = [vp, C.POINTER(Stats)]
         L.qc_batch_ep_handle.argtypes = [vp, vp, C.POINTER(C.c_int)]
         L.qc_batch_ep_connect.argtypes = [vp, vp, vp]
+        cache = [u32, vp, vp, u32, u32, u32, u32, vp, u32, u32]
+        L.qc_paged_append.argtypes = cache + [vp, vp, u32, vp, vp, vp, vp]
+        L.qc_paged_attention.argtypes = cache + [vp, u32, u32, vp, vp, C.c_float, vp, vp, vp, vp]
+        L.qc_paged_evict.argtypes = cache + [vp, vp, vp, vp, vp, u32, u32, vp, vp]
+        L.qc_logprobs.argtypes = [vp, u32, u32, u64, vp, u32, u32, vp, vp, vp, vp, vp]
         _lib = L
     return _lib
 
@@ -481,6 +487,47 @@ class Batch:
             self.close()
         except Exception:
             pass
+
+
+class PagedCache:
+    """One layer's paged key-value cache (qc_paged_*): pools [n_pages][kvheads][page][head_dim] of keys and
+    values in GGML type `kind` (F32, F16 or BF16) and a table [n_seqs][max_pages] of page numbers, all
+    at device addresses that the caller owns.  Calls enqueue on `stream` (None: the default stream)."""
+
+    F32, F16, BF16 = 0, 1, 30
+
+    def __init__(self, kind: int, k_ptr: int, v_ptr: int, n_pages: int, page: int, kvheads: int, head_dim: int,
+                 table_ptr: int, n_seqs: int, max_pages: int):
+        self._a = (kind, k_ptr, v_ptr, n_pages, page, kvheads, head_dim, table_ptr, n_seqs, max_pages)
+
+    def append(self, k_ptr: int, v_ptr: int, rows: int, pos_ptr: int, seq_ptr: int | None = None,
+               weights_ptr: int | None = None, stream: int | None = None) -> None:
+        """f32 rows [rows][kvheads][head_dim] to slots pos[i] of sequences seq[i] (None: i)."""
+        _global_check(lib().qc_paged_append(*self._a, k_ptr, v_ptr, rows, seq_ptr, pos_ptr, weights_ptr, stream))
+
+    def attention(self, q_ptr: int, heads: int, rows: int, len_ptr: int, out_ptr: int, seq_ptr: int | None = None,
+                  scale: float = 0.0, lse_ptr: int | None = None, weights_ptr: int | None = None,
+                  stream: int | None = None) -> None:
+        """out[i] = softmax(scale q[i] k^T) v over slots 0..len[i]-1 of sequence seq[i] (None: i), f32
+        [rows][heads][head_dim]; scale 0: 1/sqrt(head_dim); weights: += the rows' softmax weights."""
+        _global_check(lib().qc_paged_attention(*self._a, q_ptr, heads, rows, seq_ptr, len_ptr, scale, out_ptr, lse_ptr,
+                                               weights_ptr, stream))
+
+    def evict(self, weights_ptr: int, len_ptr: int, keep: int, recent: int, kept_ptr: int, new_len_ptr: int,
+              weights_out_ptr: int | None = None, dst_table_ptr: int | None = None, stream: int | None = None) -> None:
+        """Keep the last `recent` slots and the largest weights of the others, `keep` in all (None for
+        weights_out, dst_table: in place)."""
+        _global_check(lib().qc_paged_evict(*self._a, dst_table_ptr, weights_ptr, weights_out_ptr or weights_ptr, len_ptr,
+                                           new_len_ptr, keep, recent, kept_ptr, stream))
+
+
+def logprobs(logits_ptr: int, rows: int, n: int, stride: int | None = None, ids_ptr: int | None = None, n_ids: int = 0,
+             top: int = 0, logprobs_ptr: int | None = None, entropy_ptr: int | None = None,
+             top_ids_ptr: int | None = None, top_logprobs_ptr: int | None = None, stream: int | None = None) -> None:
+    """qc_logprobs on device arrays: log probabilities of [rows][n_ids] given ids, the entropy and the
+    `top` likeliest ids of each f32 logits row."""
+    _global_check(lib().qc_logprobs(logits_ptr, rows, n, n if stride is None else stride, ids_ptr, n_ids, top,
+                                    logprobs_ptr, entropy_ptr, top_ids_ptr, top_logprobs_ptr, stream))
 
 
 class Matrix:

@@ -209,6 +209,83 @@ pub mod ffi {
         pub fn qc_batch_ep_handle(b: *mut qc_batch, handle: *mut c_void, device_id: *mut c_int) -> c_int;
         pub fn qc_batch_ep_connect(b: *mut qc_batch, handles: *const c_void, device_ids: *const c_int) -> c_int;
 
+        pub fn qc_paged_append(
+            kind: u32,
+            k_pages: *mut c_void,
+            v_pages: *mut c_void,
+            n_pages: u32,
+            page: u32,
+            kvheads: u32,
+            head_dim: u32,
+            table: *const u32,
+            n_seqs: u32,
+            max_pages: u32,
+            k: *const c_float,
+            v: *const c_float,
+            rows: u32,
+            seq: *const u32,
+            pos: *const u32,
+            weights: *mut c_float,
+            stream: *mut c_void,
+        ) -> c_int;
+        pub fn qc_paged_attention(
+            kind: u32,
+            k_pages: *const c_void,
+            v_pages: *const c_void,
+            n_pages: u32,
+            page: u32,
+            kvheads: u32,
+            head_dim: u32,
+            table: *const u32,
+            n_seqs: u32,
+            max_pages: u32,
+            q: *const c_float,
+            heads: u32,
+            rows: u32,
+            seq: *const u32,
+            len: *const u32,
+            scale: c_float,
+            out: *mut c_float,
+            lse: *mut c_float,
+            weights: *mut c_float,
+            stream: *mut c_void,
+        ) -> c_int;
+        pub fn qc_paged_evict(
+            kind: u32,
+            k_pages: *mut c_void,
+            v_pages: *mut c_void,
+            n_pages: u32,
+            page: u32,
+            kvheads: u32,
+            head_dim: u32,
+            table: *const u32,
+            n_seqs: u32,
+            max_pages: u32,
+            dst_table: *const u32,
+            weights: *const c_float,
+            weights_out: *mut c_float,
+            len: *const u32,
+            new_len: *mut u32,
+            keep: u32,
+            recent: u32,
+            kept: *mut u32,
+            stream: *mut c_void,
+        ) -> c_int;
+        pub fn qc_logprobs(
+            logits: *const c_float,
+            rows: u32,
+            n: u32,
+            stride: u64,
+            ids: *const u32,
+            n_ids: u32,
+            top: u32,
+            logprobs: *mut c_float,
+            entropy: *mut c_float,
+            top_ids: *mut u32,
+            top_logprobs: *mut c_float,
+            stream: *mut c_void,
+        ) -> c_int;
+
         pub fn qc_reset(e: *mut qc_engine) -> c_int;
         pub fn qc_position(e: *const qc_engine, pos: *mut u32) -> c_int;
         pub fn qc_get_stats(e: *const qc_engine, out: *mut qc_stats) -> c_int;
