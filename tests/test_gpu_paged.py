@@ -35,10 +35,12 @@ def check_attention(cache, q, seq, lens, out, lse, scale=None, weights=None, bef
     # independent roundings: sqrt(D) of them a score of size ~1..8, 2^-24 each
     assert math.sqrt(num) <= 3e-6 * max(1e-30, math.sqrt(den)), math.sqrt(num / max(den, 1e-30))
     if weights is not None:
+        # eight heads' weights at a time are added to the slot's: half a step, 2^-24, each time
+        adds = 1 + -(-q.shape[1] // cache.kvheads // 8)
         total, bound = before.double(), torch.zeros_like(before, dtype=torch.float64)
         for i, (s, n) in enumerate(zip(seq, lens)):
             total[s, :, :n] += w[i]
-            bound[s, :, :n] += ew[i] + 2.0 ** -23 * (total[s, :, :n] + ew[i])
+            bound[s, :, :n] += ew[i] + adds * 2.0 ** -24 * (total[s, :, :n] + ew[i])
         err = (weights.double() - total).abs()
         assert bool((err <= bound).all()), float((err - bound).max())
 
