@@ -2096,7 +2096,7 @@ qc::PagedKV paged_kv(uint32_t kind, void* k, void* v, uint32_t n_pages, uint32_t
   ensure(head_dim >= per16 && head_dim <= 256 && head_dim % per16 == 0,
          "cache rows must be a multiple of 16 bytes and at most 256 values");
   ensure((uint64_t)max_pages * page <= 0x7fffffffull, "more than 2^31 - 1 slots in a sequence");
-  ensure(kvheads <= 0x10000 && (uint64_t)n_pages * page <= 0xffffffffull / kvheads, "more than 2^32 - 1 rows in a pool");
+  ensure(kvheads <= 0xffff && (uint64_t)n_pages * page <= 0xffffffffull / kvheads, "more than 2^32 - 1 rows in a pool");
   ensure((uint64_t)n_seqs * kvheads <= 0x7fffffffull, "too many sequences");
   return qc::PagedKV{kind, k, v, n_pages, page, kvheads, head_dim, table, n_seqs, max_pages};
 }

@@ -17,16 +17,6 @@
 namespace qc {
 namespace {
 
-constexpr uint32_t kMaxD = 256;
-
-template <class T>
-__device__ __forceinline__ float to_float(T x);
-template <>
-__device__ __forceinline__ float to_float<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <class T>
 __device__ __forceinline__ T from_float(float x);
 template <>
@@ -80,6 +70,7 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __
 // known; tiles beyond that room are scored again.
 
 constexpr int kTile = 16;
+constexpr int kMaxCluster = 16;
 
 template <class T, int DP>
 struct Att {
@@ -88,12 +79,14 @@ struct Att {
   static constexpr int kQP = sizeof(T) == 4 ? 2 : (__is_same(T, __half) ? 2 : 3);  // planes of q and of p
   static constexpr int kRow = DP * (int)sizeof(T) + 16;            // bytes of a tile row: odd multiples of 16 bytes
   static constexpr int kStage = 2 * kTile * kRow;                  //   apart, so 8 rows never share a bank
-  static constexpr int kRoom = 112 * 1024;                         // two blocks on an SM
-  static constexpr int W = 12 * kStage <= kRoom ? 4 : 2;
+  static constexpr int kRoom = 70 * 1024;                          // three blocks on an SM
+  static constexpr int W = 8 * kStage <= kRoom ? 4 : 2;
   static constexpr int kFit = kRoom / (W * kStage);
   static constexpr int NS = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
   static constexpr int kRing = W * NS * kStage;
-  static constexpr int kFixed = kRing + 8 * DP * 4 + 128;          // ring, the block's O, maxima, sums, flag
+  static constexpr int kO = DP + 4;                                // floats between two heads' O in a warp's part
+  // ring; this block's share of every block's O; every block's 8 maxima, 8 sums and flag; the warps' maxima
+  static constexpr int kFixed = kRing + 8 * DP * 4 + kMaxCluster * 17 * 4 + W * 8 * 4;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -163,16 +156,6 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[P])
   }
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -182,18 +165,18 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t a, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster(uint32_t a, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(a)
+__device__ __forceinline__ void st_cluster4(uint32_t a, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
-  return v;
+}
+// 2^x to 2 ulp (results below 2^-126 are 0)
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // One warp's query operand: the B fragments of q^T for 8 heads, and the factor that undoes q's scaling
@@ -201,28 +184,49 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
 template <class T, int DP>
 struct Query {
   using A = Att<T, DP>;
+  float raw[A::kKS][A::kF32 ? 2 : 4];
   uint32_t f[A::kKS][A::kQP][2];
   float undo0, undo1;
 
-  // q: head 0 of the group; heads >= G and values >= D are zero.  factor: scale log2 e.
-  __device__ __forceinline__ void load(const float* q, uint32_t D, uint32_t G, float factor) {
+  // Starts reading q (head 0 of the group); heads >= G and values >= D are zero.
+  __device__ __forceinline__ void fetch(const float* q, uint32_t D, uint32_t G) {
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
     const float* qr = q + (uint64_t)g * D;
+#pragma unroll
+    for (int k = 0; k < A::kKS; k++)
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        if constexpr (A::kF32) {
+          const uint32_t d = k * 8 + b * 4 + t;
+          raw[k][b] = g < G && d < D ? qr[d] : 0.f;
+        } else {
+          const uint32_t d = k * 16 + b * 8 + 2 * t;
+          float2 x = make_float2(0.f, 0.f);
+          if (g < G && d < D) x = *reinterpret_cast<const float2*>(qr + d);
+          raw[k][2 * b] = x.x;
+          raw[k][2 * b + 1] = x.y;
+        }
+      }
+  }
+  // Splits q times factor (scale log2 e) into planes.
+  __device__ __forceinline__ void split(float factor) {
+    const uint32_t t = threadIdx.x & 3;
     undo0 = undo1 = 1.f;
     if constexpr (A::kF32) {
 #pragma unroll
-      for (int k = 0; k < A::kKS; k++)
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const uint32_t d = k * 8 + b * 4 + t;
-          split_tf32(g < G && d < D ? qr[d] * factor : 0.f, f[k][0][b], f[k][1][b]);
-        }
+      for (int k = 0; k < A::kKS; k++) {
+        const float x = raw[k][0] * factor, y = raw[k][1] * factor;
+        split_tf32(x, f[k][0][0], f[k][1][0]);
+        split_tf32(y, f[k][0][1], f[k][1][1]);
+      }
     } else {
       float up = 1.f;
       if constexpr (__is_same(T, __half)) {  // the largest |q| of a head to 2^13..2^14: two planes hold 22 bits
         float mx = 0.f;
-        if (g < G)
-          for (uint32_t d = t; d < D; d += 4) mx = fmaxf(mx, fabsf(qr[d] * factor));
+#pragma unroll
+        for (int k = 0; k < A::kKS; k++)
+#pragma unroll
+          for (int b = 0; b < 4; b++) mx = fmaxf(mx, fabsf(raw[k][b] * factor));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
@@ -233,17 +237,18 @@ struct Query {
         undo1 = __shfl_sync(0xffffffffu, down, 8 * t + 4);
       }
 #pragma unroll
-      for (int k = 0; k < A::kKS; k++)
+      for (int k = 0; k < A::kKS; k++) {
+        const float x[4] = {raw[k][0] * factor * up, raw[k][1] * factor * up, raw[k][2] * factor * up,
+                            raw[k][3] * factor * up};
+        uint32_t lo[A::kQP], hi[A::kQP];
+        split_pair<T, A::kQP>(x[0], x[1], lo);
+        split_pair<T, A::kQP>(x[2], x[3], hi);
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const uint32_t d = k * 16 + b * 8 + 2 * t;
-          float2 x = make_float2(0.f, 0.f);
-          if (g < G && d < D) x = *reinterpret_cast<const float2*>(qr + d);
-          uint32_t pl[A::kQP];
-          split_pair<T, A::kQP>(x.x * factor * up, x.y * factor * up, pl);
-#pragma unroll
-          for (int p = 0; p < A::kQP; p++) f[k][p][b] = pl[p];
+        for (int p = 0; p < A::kQP; p++) {
+          f[k][p][0] = lo[p];
+          f[k][p][1] = hi[p];
         }
+      }
     }
   }
 
@@ -344,22 +349,26 @@ __device__ __forceinline__ void add_values(uint32_t vtile, const float (&p)[4], 
   }
 }
 
+// How a launch splits a sequence: 2^logc blocks a cluster; a warp's next tile lies step_pages pages and
+// step_slots slots further; with weights, the tiles a warp keeps the scores of.
+struct AttSplit {
+  uint32_t logc, step_pages, step_slots, score_tiles;
+};
+
 template <class T, int DP, bool WEIGHTS>
-__global__ void __launch_bounds__(Att<T, DP>::W * 32) k_paged_attention(PagedKV c, PagedRows r, uint32_t score_tiles) {
+__global__ void __launch_bounds__(Att<T, DP>::W * 32, Att<T, DP>::kFixed <= 75 * 1024 ? 3 : 1)
+    k_paged_attention(PagedKV c, PagedRows r, AttSplit sp) {
   using A = Att<T, DP>;
   constexpr int W = A::W, NS = A::NS;
   extern __shared__ __align__(16) uint8_t sm[];
-  float* const block_o = reinterpret_cast<float*>(sm + A::kRing);  // [8][DP]
-  float* const block_m = block_o + 8 * DP;                         // [8]
-  float* const block_l = block_m + 8;                              // [8]
-  uint32_t* const block_bad = reinterpret_cast<uint32_t*>(block_l + 8);
-  const uint32_t C = cluster_size(), rank = cluster_rank();
-  const uint32_t unit = blockIdx.x / C, h = unit % c.kvheads, first = unit / c.kvheads;
+  float* const in_o = reinterpret_cast<float*>(sm + A::kRing);  // [C][8 DP / C]: this block's share of every block's O
+  float* const in_m = in_o + 8 * DP;                            // [C][17]: every block's maxima, sums, flag
+  float* const warp_m = in_m + kMaxCluster * 17;                // [W][8]
+  const uint32_t C = 1u << sp.logc, rank = blockIdx.x & (C - 1), h = blockIdx.y, first = blockIdx.x >> sp.logc;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
   uint8_t* const ring = sm + warp * NS * A::kStage;
   const uint32_t ring_a = smem_addr(ring);
-  float* const mine = reinterpret_cast<float*>(ring);  // the warp's O [8][DP], maxima and sums, once its tiles are done
   const uint32_t s = r.seq ? r.seq[first] : first;
   if (s >= c.n_seqs) return;  // (the whole cluster)
   if (WEIGHTS && r.seq) {     // the cluster of a sequence's first row takes all its rows, in order
@@ -368,63 +377,108 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32) k_paged_attention(PagedKV 
     if (__syncthreads_or(earlier)) return;
   }
   const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
+  // Where pages hold whole runs of 8 positions (RUNS) a lane copies its part of a run with one address;
+  // else every position has its own page and its lanes ask the lane that looked it up.
+  const bool runs = c.page % 8 == 0;
+  const uint32_t step = C * W * kTile, gw = rank * W + warp;
+  const uint32_t ahead = runs ? lane / 16 * 8 : lane % kTile;  // the position of a tile this lane looks up
+  const uint32_t page0 = (gw * kTile + ahead) / c.page, slot0 = (gw * kTile + ahead) % c.page;
+  bool again = false;
 
   for (uint32_t i = first; i < r.rows; i++) {
     if (i > first && !(WEIGHTS && r.seq)) break;
     if (i > first && r.seq[i] != s) continue;
     const uint32_t len = r.len[i];
     const bool too_long = len > cap;
-    const uint32_t tiles = too_long ? 0 : (len + kTile - 1) / kTile, gw = rank * W + warp;
+    const uint32_t tiles = too_long ? 0 : (len + kTile - 1) / kTile;
     const uint32_t mine_n = tiles > gw ? (tiles - gw + C * W - 1) / (C * W) : 0;  // this warp's tiles
     for (uint32_t g0 = 0; g0 < G; g0 += 8) {
       const uint32_t gn = min(8u, G - g0);
       bool bad = false;
-      if (chunks * 16 < DP * sizeof(T)) {  // columns D.. of the tiles are zero (the join below writes over them)
+      Query<T, DP> q;
+      q.fetch(r.q + ((uint64_t)i * r.heads + h * G + g0) * D, D, gn);
+      auto clear_columns = [&](uint32_t rows) {  // columns D.. of the tiles are zero (the join writes over them)
         const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
-        for (uint32_t e = lane; e < 2 * NS * kTile * extra; e += 32)
+        for (uint32_t e = lane; e < rows * extra; e += 32)
           *reinterpret_cast<uint4*>(ring + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
-      }
-      // The pool row of position lane (< 16) of this warp's n-th tile; kNoSlot: nothing to read.
-      auto row_of = [&](uint32_t n) {
-        const uint32_t j = (gw + n * C * W) * kTile + lane % kTile;
-        if (n >= mine_n || j >= len) return kNoSlot;
-        const uint32_t p = pages[j / c.page];
+      };
+      // The page number of position j, table entry `at`, and its row at slot `in` for the tile from j0 on.
+      auto page_at = [&](uint32_t j, uint32_t at) { return j < len && !too_long ? pages[at] : kNoSlot; };
+      auto row_of = [&](uint32_t p, uint32_t in, uint32_t j0) {
         if (p >= c.n_pages) {
-          bad = true;
+          bad |= j0 + ahead < len;
           return kNoSlot;
         }
-        return (p * c.kvheads + h) * c.page + j % c.page;
+        return (p * c.kvheads + h) * c.page + in;
       };
-      auto fetch = [&](uint32_t slot, uint32_t row, bool with_v) {
-        const uint32_t dst = ring_a + slot * A::kStage;
+      // Copies the tile of positions j0.. into a ring slot; row: this lane's lookup.
+      auto fetch = [&](uint32_t slot, uint32_t row, uint32_t j0, bool with_v) {
         constexpr uint32_t kCh = DP * sizeof(T) / 16;
+        const uint32_t dst = ring_a + slot * A::kStage;
+        const uint8_t *kp = static_cast<const uint8_t*>(c.k), *vp = static_cast<const uint8_t*>(c.v);
+        if (runs) {
+          const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0), row1 = __shfl_sync(0xffffffffu, row, 16);
+          const uint64_t bytes = D * sizeof(T);
+          const uint64_t at0 = row0 == kNoSlot ? 0 : row0 * bytes, at1 = (row1 == kNoSlot ? 0 : row1 * bytes) - 8 * bytes;
+          const uint32_t n = j0 < len ? len - j0 : 0, n0 = row0 == kNoSlot ? 0 : n, n1 = row1 == kNoSlot ? 0 : n;
+#pragma unroll
+          for (uint32_t e0 = 0; e0 < kTile * kCh; e0 += 32) {
+            const uint32_t e = e0 + lane, p = e / kCh, ch = e % kCh;
+            const bool second = e0 >= 8 * kCh;
+            const uint64_t o = (second ? at1 : at0) + (p * chunks + ch) * 16;
+            const bool real = p < (second ? n1 : n0);
+            if (DP * sizeof(T) != chunks * 16 && ch >= chunks) continue;
+            copy16(dst + p * A::kRow + ch * 16, kp + o, real);
+            if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, real);
+          }
+        } else {
 #pragma unroll 4
-        for (uint32_t e = lane; e < kTile * kCh; e += 32) {
-          const uint32_t p = e / kCh, ch = e % kCh;
-          const uint32_t from = __shfl_sync(0xffffffffu, row, p);
-          const uint64_t at = from == kNoSlot ? 0 : (uint64_t)from * D * sizeof(T) + ch * 16;
-          if (ch >= chunks) continue;
-          copy16(dst + p * A::kRow + ch * 16, static_cast<const uint8_t*>(c.k) + at, from != kNoSlot);
-          if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, static_cast<const uint8_t*>(c.v) + at, from != kNoSlot);
+          for (uint32_t e = lane; e < kTile * kCh; e += 32) {
+            const uint32_t p = e / kCh, ch = e % kCh;
+            const uint32_t from = __shfl_sync(0xffffffffu, row, p);
+            const uint64_t o = from == kNoSlot ? 0 : (uint64_t)from * D * sizeof(T) + ch * 16;
+            if (ch >= chunks) continue;
+            copy16(dst + p * A::kRow + ch * 16, kp + o, from != kNoSlot);
+            if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, from != kNoSlot);
+          }
         }
       };
+      // this warp's tiles one after the other
+      uint32_t j = gw * kTile + ahead, at = page0, in = slot0;
+      auto advance = [&] {
+        j += step;
+        at += sp.step_pages;
+        in += sp.step_slots;
+        if (in >= c.page) {
+          in -= c.page;
+          at++;
+        }
+      };
+      uint32_t pg[NS], slots[NS];
 #pragma unroll
       for (int n = 0; n < NS; n++) {
-        fetch(n, row_of(n), true);
-        copy_commit();
+        pg[n] = page_at(j, at);
+        slots[n] = in;
+        advance();
       }
-      uint32_t next = row_of(NS);
-      Query<T, DP> q;
-      q.load(r.q + ((uint64_t)i * r.heads + h * G + g0) * D, D, gn, r.scale * 1.4426950408889634f);
+      uint32_t next = page_at(j, at), next_in = in, j0 = gw * kTile;
+      if (chunks * 16 < DP * sizeof(T)) clear_columns(2 * NS * kTile);
+#pragma unroll
+      for (int n = 0; n < NS; n++) {
+        fetch(n, row_of(pg[n], slots[n], j0), j0, true);
+        copy_commit();
+        j0 += step;
+      }
+      q.split(r.scale * 1.4426950408889634f);
       float o[DP / 16][4], m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
 #pragma unroll
       for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
-      float4* const kept_scores = reinterpret_cast<float4*>(sm + A::kFixed) + (uint64_t)warp * score_tiles * 32 + lane;
+      float4* const kept_scores = reinterpret_cast<float4*>(sm + A::kFixed) + (uint64_t)warp * sp.score_tiles * 32 + lane;
       auto masked_scores = [&](uint32_t n, uint32_t ktile, float (&x)[4]) {
         q.scores(ktile, x);
-        const uint32_t j = (gw + n * C * W) * kTile + g;
-        if (j >= len) x[0] = x[1] = -INFINITY;
-        if (j + 8 >= len) x[2] = x[3] = -INFINITY;
+        const uint32_t pos = gw * kTile + n * step + g;
+        if (pos >= len) x[0] = x[1] = -INFINITY;
+        if (pos + 8 >= len) x[2] = x[3] = -INFINITY;
       };
       for (uint32_t n = 0, slot = 0; n < mine_n; n++, slot = slot + 1 == NS ? 0 : slot + 1) {
         copy_wait<NS - 1>();
@@ -432,7 +486,7 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32) k_paged_attention(PagedKV 
         const uint32_t tile_a = ring_a + slot * A::kStage;
         float x[4];
         masked_scores(n, tile_a, x);
-        if (WEIGHTS && n < score_tiles) kept_scores[n * 32] = make_float4(x[0], x[1], x[2], x[3]);
+        if (WEIGHTS && n < sp.score_tiles) kept_scores[n * 32] = make_float4(x[0], x[1], x[2], x[3]);
         const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
         if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
           float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
@@ -441,7 +495,7 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32) k_paged_attention(PagedKV 
             n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
             n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
           }
-          const float f0 = exp2f(m0 - n0), f1 = exp2f(m1 - n1);
+          const float f0 = pow2(m0 - n0), f1 = pow2(m1 - n1);
           m0 = n0;
           m1 = n1;
           l0 *= f0;
@@ -454,131 +508,160 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32) k_paged_attention(PagedKV 
             y[3] *= f1;
           }
         }
-        const float p[4] = {exp2f(x[0] - m0), exp2f(x[1] - m1), exp2f(x[2] - m0), exp2f(x[3] - m1)};
+        const float p[4] = {pow2(x[0] - m0), pow2(x[1] - m1), pow2(x[2] - m0), pow2(x[3] - m1)};
         l0 += p[0] + p[2];
         l1 += p[1] + p[3];
         add_values<T, DP>(tile_a + kTile * A::kRow, p, o);
         __syncwarp();
-        fetch(slot, next, true);
+        fetch(slot, row_of(next, next_in, j0), j0, true);
         copy_commit();
-        next = row_of(n + NS + 1);
+        j0 += step;
+        advance();
+        next = page_at(j, at);
+        next_in = in;
       }
       copy_wait<0>();
-      __syncwarp();
-      // the warps of the block
+      // the warps of the block: O and sums relative to the block's maxima, then added up
 #pragma unroll
       for (int w = 4; w < 32; w *= 2) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, w);
         l1 += __shfl_xor_sync(0xffffffffu, l1, w);
       }
+      if (g == 0) {
+        warp_m[warp * 8 + 2 * t] = m0;
+        warp_m[warp * 8 + 2 * t + 1] = m1;
+      }
+      bad = __syncthreads_or(bad) || too_long;
+      float M0 = m0, M1 = m1;
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        M0 = fmaxf(M0, warp_m[w * 8 + 2 * t]);
+        M1 = fmaxf(M1, warp_m[w * 8 + 2 * t + 1]);
+      }
+      const float f0 = pow2(m0 - M0), f1 = pow2(m1 - M1);
+      float* const mine = reinterpret_cast<float*>(ring);  // [8][kO], sums
 #pragma unroll
       for (int m = 0; m < DP / 16; m++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) mine[(2 * t + e % 2) * DP + m * 16 + g + (e / 2) * 8] = o[m][e];
+        for (int e = 0; e < 4; e++)
+          mine[(2 * t + e % 2) * A::kO + m * 16 + g + (e / 2) * 8] = o[m][e] * (e % 2 ? f1 : f0);
       if (g == 0) {
-        mine[8 * DP + 2 * t] = m0;
-        mine[8 * DP + 2 * t + 1] = m1;
-        mine[8 * DP + 8 + 2 * t] = l0;
-        mine[8 * DP + 8 + 2 * t + 1] = l1;
+        mine[8 * A::kO + 2 * t] = l0 * f0;
+        mine[8 * A::kO + 2 * t + 1] = l1 * f1;
       }
-      bad = __syncthreads_or(bad) || too_long;
+      if (again) cluster_sync();  // the other blocks have read what was sent for the previous turn
+      else __syncthreads();
+      again = true;
+      // what they add up to goes to the blocks of the cluster: a share of O to each, maxima and sums to all
       auto part = [&](uint32_t w) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage); };
-      for (uint32_t e = tid; e < 8 * DP / 4; e += W * 32) {
-        const uint32_t hh = e / (DP / 4);
-        float M = -FLT_MAX;
-#pragma unroll
-        for (int w = 0; w < W; w++) M = fmaxf(M, part(w)[8 * DP + hh]);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-          const float f = exp2f(part(w)[8 * DP + hh] - M);
-          const float4 y = reinterpret_cast<const float4*>(part(w))[e];
-          sum.x = fmaf(y.x, f, sum.x);
-          sum.y = fmaf(y.y, f, sum.y);
-          sum.z = fmaf(y.z, f, sum.z);
-          sum.w = fmaf(y.w, f, sum.w);
-        }
-        reinterpret_cast<float4*>(block_o)[e] = sum;
-        if (e % (DP / 4) == 0) {
-          float L = 0.f;
-#pragma unroll
-          for (int w = 0; w < W; w++) L = fmaf(part(w)[8 * DP + 8 + hh], exp2f(part(w)[8 * DP + hh] - M), L);
-          block_m[hh] = M;
-          block_l[hh] = L;
-        }
-      }
-      if (tid == 0) *block_bad = bad;
-      // the blocks of the cluster: each sums a share of the outputs over all blocks
-      cluster_sync();
-      const uint32_t o_a = smem_addr(block_o), m_a = smem_addr(block_m), l_a = smem_addr(block_l), b_a = smem_addr(block_bad);
-      bad = false;
-      for (uint32_t k = 0; k < C; k++) bad |= __float_as_uint(ld_cluster(cluster_addr(b_a, k))) != 0;
-      const float qnan = __int_as_float(0x7fc00000);
-      const uint64_t row_head = (uint64_t)i * r.heads + h * G + g0;
-      for (uint32_t e = rank * W * 32 + tid; e < gn * (DP / 4); e += C * W * 32) {
+      const uint32_t share = (2 * DP) >> sp.logc;  // 16-byte pieces of O of one block
+      for (uint32_t e = tid; e < 2 * DP; e += W * 32) {
         const uint32_t hh = e / (DP / 4), d = e % (DP / 4) * 4;
-        float M = -FLT_MAX, L = 0.f;
-        for (uint32_t k = 0; k < C; k++) M = fmaxf(M, ld_cluster(cluster_addr(m_a + hh * 4, k)));
+        float4 sum = *reinterpret_cast<const float4*>(part(0) + hh * A::kO + d);
+#pragma unroll
+        for (int w = 1; w < W; w++) {
+          const float4 y = *reinterpret_cast<const float4*>(part(w) + hh * A::kO + d);
+          sum.x += y.x;
+          sum.y += y.y;
+          sum.z += y.z;
+          sum.w += y.w;
+        }
+        const uint32_t to = e / share;
+        st_cluster4(cluster_addr(smem_addr(in_o) + (rank * share + e - to * share) * 16, to), sum);
+      }
+      for (uint32_t e = tid; e < C * 8; e += W * 32) {
+        const uint32_t hh = e % 8, to = e / 8;
+        float M = warp_m[hh], L = part(0)[8 * A::kO + hh];
+#pragma unroll
+        for (int w = 1; w < W; w++) {
+          M = fmaxf(M, warp_m[w * 8 + hh]);
+          L += part(w)[8 * A::kO + hh];
+        }
+        const uint32_t a = cluster_addr(smem_addr(in_m) + rank * 17 * 4, to);
+        st_cluster(a + hh * 4, M);
+        st_cluster(a + 32 + hh * 4, bad ? __int_as_float(0x7fc00000) : L);
+        if (hh == 0) st_cluster(a + 64, bad ? 1.f : 0.f);
+      }
+      cluster_sync();
+      // the maximum and the sum of head hh over the blocks (bad: NaN)
+      auto total = [&](uint32_t hh, float& M, float& L) {
+        M = -FLT_MAX;
+        L = 0.f;
+#pragma unroll 4
+        for (uint32_t k = 0; k < C; k++) M = fmaxf(M, in_m[k * 17 + hh]);
+#pragma unroll 4
+        for (uint32_t k = 0; k < C; k++) L = fmaf(in_m[k * 17 + 8 + hh], pow2(in_m[k * 17 + hh] - M), L);
+      };
+      const uint64_t row_head = (uint64_t)i * r.heads + h * G + g0;
+      for (uint32_t e = tid; e < share; e += W * 32) {
+        const uint32_t hh = (rank * share + e) / (DP / 4), d = (rank * share + e) % (DP / 4) * 4;
+        if (hh >= gn || d >= D) continue;
+        float M, L;
+        total(hh, M, L);
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (uint32_t k = 0; k < C; k++) {
-          const float f = exp2f(ld_cluster(cluster_addr(m_a + hh * 4, k)) - M);
-          const float4 y = ld_cluster4(cluster_addr(o_a + e * 16, k));
-          L = fmaf(ld_cluster(cluster_addr(l_a + hh * 4, k)), f, L);
+          const float f = pow2(in_m[k * 17 + hh] - M);
+          const float4 y = reinterpret_cast<const float4*>(in_o)[k * share + e];
           sum.x = fmaf(y.x, f, sum.x);
           sum.y = fmaf(y.y, f, sum.y);
           sum.z = fmaf(y.z, f, sum.z);
           sum.w = fmaf(y.w, f, sum.w);
         }
-        const float inv = bad ? qnan : L == 0.f ? 0.f : (__is_same(T, __half) ? 1.f / 16384.f : 1.f) / L;
-        if (d < D)
-          *reinterpret_cast<float4*>(r.out + (row_head + hh) * D + d) =
-              make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-        if (d == 0 && r.lse) r.lse[row_head + hh] = bad ? qnan : L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+        const float inv = L == 0.f ? 0.f : (__is_same(T, __half) ? 1.f / 16384.f : 1.f) / L;
+        *reinterpret_cast<float4*>(r.out + (row_head + hh) * D + d) =
+            make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        if (d == 0 && r.lse) r.lse[row_head + hh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
       }
-      if (WEIGHTS && !bad) {
+      if (WEIGHTS) {
+        bad = false;
+        for (uint32_t k = 0; k < C; k++) bad |= in_m[k * 17 + 16] != 0.f;
         float M[2], inv[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const uint32_t hh = 2 * t + u;
-          float L = 0.f;
-          M[u] = -FLT_MAX;
-          for (uint32_t k = 0; k < C; k++) M[u] = fmaxf(M[u], ld_cluster(cluster_addr(m_a + hh * 4, k)));
-          for (uint32_t k = 0; k < C; k++)
-            L = fmaf(ld_cluster(cluster_addr(l_a + hh * 4, k)), exp2f(ld_cluster(cluster_addr(m_a + hh * 4, k)) - M[u]), L);
-          inv[u] = hh >= gn || L == 0.f ? 0.f : 1.f / L;
+          float L;
+          total(2 * t + u, M[u], L);
+          inv[u] = 2 * t + u >= gn || L == 0.f ? 0.f : 1.f / L;
         }
-        if (mine_n > score_tiles && chunks * 16 < DP * sizeof(T)) {  // (the join has written over the zero columns)
-          const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
+        if (mine_n > sp.score_tiles && chunks * 16 < DP * sizeof(T)) {
           __syncwarp();
-          for (uint32_t e = lane; e < kTile * extra; e += 32)
-            *reinterpret_cast<uint4*>(ring + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
+          clear_columns(kTile);
         }
         float* const w = r.weights + ((uint64_t)s * c.kvheads + h) * cap;
-        for (uint32_t n = 0; n < mine_n; n++) {
-          float x[4];
-          if (n < score_tiles) {
-            const float4 y = kept_scores[n * 32];
-            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-          } else {
-            __syncwarp();
-            fetch(0, row_of(n), false);
-            copy_commit();
-            copy_wait<0>();
-            __syncwarp();
-            masked_scores(n, ring_a, x);
+        // (the weights' reads first, four tiles at a time: one after the other each would wait for the last)
+        for (uint32_t n0 = 0; n0 < mine_n && !bad; n0 += 4) {
+          float old[4];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; u++) {
+            const uint32_t pos = gw * kTile + (n0 + u) * step + g + 8 * t;
+            old[u] = t < 2 && n0 + u < mine_n && pos < len ? w[pos] : 0.f;
           }
-          float w0 = exp2f(x[0] - M[0]) * inv[0] + exp2f(x[1] - M[1]) * inv[1];
-          float w8 = exp2f(x[2] - M[0]) * inv[0] + exp2f(x[3] - M[1]) * inv[1];
-          w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
-          w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
-          w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
-          w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
-          const uint32_t j = (gw + n * C * W) * kTile + g;
-          if (t == 0 && j < len) w[j] += w0;
-          if (t == 1 && j + 8 < len) w[j + 8] += w8;
+#pragma unroll
+          for (uint32_t u = 0; u < 4; u++) {
+            const uint32_t n = n0 + u, base = gw * kTile + n * step, pos = base + ahead;
+            if (n >= mine_n) break;
+            float x[4];
+            if (n < sp.score_tiles) {
+              const float4 y = kept_scores[n * 32];
+              x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+            } else {
+              __syncwarp();
+              fetch(0, row_of(page_at(pos, pos / c.page), pos % c.page, base), base, false);
+              copy_commit();
+              copy_wait<0>();
+              __syncwarp();
+              masked_scores(n, ring_a, x);
+            }
+            float w0 = pow2(x[0] - M[0]) * inv[0] + pow2(x[1] - M[1]) * inv[1];
+            float w8 = pow2(x[2] - M[0]) * inv[0] + pow2(x[3] - M[1]) * inv[1];
+            w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+            w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
+            w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+            w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
+            if (t < 2 && base + g + 8 * t < len) w[base + g + 8 * t] = old[u] + (t ? w8 : w0);
+          }
         }
       }
-      cluster_sync();  // the other blocks have read this one's part
     }
   }
 }
@@ -694,7 +777,6 @@ cudaError_t launch_paged_append(const PagedKV& c, const float* k, const float* v
 
 namespace {
 
-constexpr int kMaxCluster = 16;
 constexpr uint32_t kMaxAttSmem = 220 * 1024;
 
 template <class T, int DP, bool WEIGHTS>
@@ -706,33 +788,37 @@ cudaError_t att_prepare() {
   return e;
 }
 
-// Blocks of a cluster: enough that the launch fills the GPU (two blocks an SM) several times over, as the
-// sequences' lengths differ and are not known here, as long as a warp keeps two tiles of a full cache.
+// Blocks of a cluster: enough that the launch fills the GPU (three blocks an SM) twice over, as the
+// sequences' lengths differ and are not known here, as long as a warp keeps four tiles of a full cache.
 template <class T, int DP, bool WEIGHTS>
 cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   using A = Att<T, DP>;
   const uint32_t units = r.rows * c.kvheads, tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
-  uint32_t C = 1;
-  while (C < (uint32_t)kMaxCluster && (uint64_t)units * C < 1024 && tiles >= 4 * C * A::W) C *= 2;
-  uint32_t keep = 0;
+  AttSplit sp{};
+  while (sp.logc < 4 && tiles > A::W << sp.logc &&
+         ((units << sp.logc) < 148 || ((units << sp.logc) < 1024 && tiles >= (12 * A::W) << sp.logc)))
+    sp.logc++;
   if (WEIGHTS) {
     const uint32_t room = (kMaxAttSmem - A::kFixed) / (A::W * 512);
-    while (C < (uint32_t)kMaxCluster && (tiles + C * A::W - 1) / (C * A::W) > room) C *= 2;
-    keep = (tiles + C * A::W - 1) / (C * A::W);
-    keep = keep < room ? keep : room;
+    auto per_warp = [&] { return (tiles + (A::W << sp.logc) - 1) / (A::W << sp.logc); };
+    while (sp.logc < 4 && per_warp() > room) sp.logc++;
+    sp.score_tiles = per_warp() < room ? per_warp() : room;
   }
+  const uint32_t step = (A::W * kTile) << sp.logc;
+  sp.step_pages = step / c.page;
+  sp.step_slots = step % c.page;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(units * C);
+  cfg.gridDim = dim3(r.rows << sp.logc, c.kvheads);
   cfg.blockDim = dim3(A::W * 32);
-  cfg.dynamicSmemBytes = A::kFixed + keep * A::W * 512;
+  cfg.dynamicSmemBytes = A::kFixed + sp.score_tiles * A::W * 512;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.x = 1u << sp.logc;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS>, c, r, keep);
+  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS>, c, r, sp);
 }
 
 // Rows are computed at the next of these widths; the columns between are zeros in shared memory.
