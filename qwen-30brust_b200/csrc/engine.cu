@@ -66,6 +66,7 @@ void prepare_device(int device) {
   QC_CK(qc::batch_prepare(kMaxSmem));
   QC_CK(qc::qgemm_prepare());
   QC_CK(qc::paged_prepare());
+  QC_CK(qc::logprobs_prepare());
   done[device] = true;
 }
 

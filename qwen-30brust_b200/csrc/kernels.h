@@ -345,6 +345,7 @@ struct LogprobArgs {
   float* top_logprobs;
 };
 constexpr uint32_t kMaxTop = 64;
+cudaError_t logprobs_prepare();
 cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st);
 
 // n keystream words of the sampler (advancing it), for reproducibility checks.
