@@ -269,8 +269,8 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
  * 0..keep-1 of the pages dst_table[s] ([n_seqs][max_pages]; NULL: in place) and to weights_out (may be
  * weights).  kept ([n_seqs][kvheads][keep]) receives the slots' old numbers (0xffffffff behind the last
  * one), new_len (may be len) min(len, keep).  A sequence within keep keeps all slots (and is copied
- * where dst_table names other pages).  Pages of dst_table are written by one sequence only, and are
- * either not read by this call or, in place, the same pages at the same places. */
+ * where dst_table names other pages).  A page of dst_table belongs to one sequence and is not read by
+ * this call; in place (dst_table NULL or the table itself) a sequence's pages are its own. */
 int qc_paged_evict(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages, uint32_t page, uint32_t kvheads,
                    uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages, const uint32_t* dst_table,
                    const float* weights, float* weights_out, const uint32_t* len, uint32_t* new_len, uint32_t keep,

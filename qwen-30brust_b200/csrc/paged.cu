@@ -673,91 +673,210 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ uint32_t block_sum(uint32_t x, uint32_t* tmp) {
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = 0;
-  for (uint32_t w = 0; w < blockDim.x / 32; w++) x += tmp[w];
-  return x;
-}
+constexpr uint32_t kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr uint32_t kSelHold = 40960;  // slots whose weights a block holds in shared memory
+constexpr uint32_t kHists = 4, kBins = 2048;
 
 // The slots that (sequence, KV head) keeps, ascending, to kept[..][keep]; kNoSlot behind them, and in
-// the first place when the sequence's length or pages are invalid.
-__global__ void __launch_bounds__(1024) k_evict_select(PagedKV c, PagedEvict e) {
-  __shared__ uint32_t tmp[32], s_bad, s_at;
-  const uint32_t s = blockIdx.x / c.kvheads, tid = threadIdx.x;
+// the first place when the sequence's length or pages are invalid.  Their weights to weights_out.
+//
+// The want-th largest key is found by its first 11, next 11 and last 10 bits: a histogram of the keys that
+// share the bits found so far (four, for every fourth lane: the first bits bunch up), then a scan over its
+// bins.  Then the slots above it and the first ones at it are numbered: each thread counts its run of
+// slots, and knows its place from the counts of those before.  The weights are read once, and held in shared memory; of a
+// sequence of more than kSelHold slots they are read again for each turn.
+__global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEvict e, uint32_t hold) {
+  extern __shared__ float held[];  // [hold]
+  __shared__ uint32_t hist[kHists][kBins];
+  __shared__ uint32_t warp_n[2][kSelWarps];
+  __shared__ uint32_t s_bin, s_left;
+  const uint32_t s = blockIdx.x / c.kvheads, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t n = e.len[s], cap = c.max_pages * c.page, m = min(n, e.keep);
-  uint32_t* kept = e.kept + (uint64_t)blockIdx.x * e.keep;
-  if (tid == 0) {
-    s_bad = n > cap;
-    s_at = 0;
-  }
-  __syncthreads();
-  if (n <= cap) {
-    for (uint32_t p = tid; p < (n + c.page - 1) / c.page; p += blockDim.x)
-      if (c.table[(uint64_t)s * c.max_pages + p] >= c.n_pages) s_bad = 1;
-    for (uint32_t p = tid; p < (m + c.page - 1) / c.page; p += blockDim.x)
-      if (e.dst_table[(uint64_t)s * c.max_pages + p] >= c.n_pages) s_bad = 1;
-  }
-  __syncthreads();
-  if (s_bad || n <= e.keep) {
-    for (uint32_t i = tid; i < e.keep; i += blockDim.x) kept[i] = !s_bad && i < n ? i : kNoSlot;
-    return;
-  }
-  const float* w = e.weights + (uint64_t)blockIdx.x * cap;
-  const uint32_t old = n - e.recent, want = e.keep - e.recent;
-  uint32_t T = 0;  // the want-th largest key
-  for (int b = 31; b >= 0 && want; b--) {
-    const uint32_t cand = T | 1u << b;
-    uint32_t cnt = 0;
-    for (uint32_t i = tid; i < old; i += blockDim.x) cnt += weight_key(w[i]) >= cand;
-    if (block_sum(cnt, tmp) >= want) T = cand;
-  }
-  uint32_t above = 0;
-  for (uint32_t i = tid; i < old; i += blockDim.x) above += weight_key(w[i]) > T;
-  uint32_t ties = want - block_sum(above, tmp);  // slots with key T that stay: the first ones
-  if (!want) ties = 0;
-  __syncthreads();
-  if (tid == 0)
-    for (uint32_t i = 0; i < n; i++) {
-      const uint32_t key = i < old ? weight_key(w[i]) : 0;
-      bool take = i >= old || (want && key > T);
-      if (i < old && want && key == T && ties) {
-        take = true;
-        ties--;
-      }
-      if (take) kept[s_at++] = i;
-    }
-}
-
-// Rows kept[i] of K (blockIdx.y 0) or V (1) and their weights to slot i.  In place this is a move to
-// lower slots: kept[i] >= i ascending, so a tile may be written once it has been read.
-template <class T>
-__global__ void __launch_bounds__(256) k_evict_move(PagedKV c, PagedEvict e) {
-  const uint32_t s = blockIdx.x / c.kvheads, h = blockIdx.x % c.kvheads, D = c.D, cap = c.max_pages * c.page;
-  const uint32_t* kept = e.kept + (uint64_t)blockIdx.x * e.keep;
-  if (kept[0] == kNoSlot) {  // nothing cached, or an invalid sequence
-    if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) e.new_len[s] = e.len[s];
-    return;
-  }
-  const uint32_t m = min(e.len[s], e.keep);
-  T* pool = static_cast<T*>(blockIdx.y ? c.v : c.k);
+  uint32_t* const kept = e.kept + (uint64_t)blockIdx.x * e.keep;
   const float* w = e.weights + (uint64_t)blockIdx.x * cap;
   float* wo = e.weights_out + (uint64_t)blockIdx.x * cap;
-  for (uint32_t i = 0; i < m; i++) {
-    const uint64_t from = pool_row(c, c.table, s, h, kept[i]), to = pool_row(c, e.dst_table, s, h, i);
-    T x{};
-    float y = 0.f;
-    if (threadIdx.x < D) x = pool[from * D + threadIdx.x];
-    if (threadIdx.x == 0 && !blockIdx.y) y = w[kept[i]];
+  bool bad = n > cap;
+  if (!bad) {
+    for (uint32_t p = tid; p < (n + c.page - 1) / c.page; p += kSelThreads)
+      bad |= c.table[(uint64_t)s * c.max_pages + p] >= c.n_pages;
+    for (uint32_t p = tid; p < (m + c.page - 1) / c.page; p += kSelThreads)
+      bad |= e.dst_table[(uint64_t)s * c.max_pages + p] >= c.n_pages;
+  }
+  const bool all = n <= e.keep, fits = n <= hold;
+  auto hold_weights = [&](uint32_t from, uint32_t count) {  // (eight reads on their way at a time)
+    for (uint32_t i0 = tid; i0 < count; i0 += 8 * kSelThreads) {
+      float x[8];
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) x[u] = i0 + u * kSelThreads < count ? w[from + i0 + u * kSelThreads] : 0.f;
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++)
+        if (i0 + u * kSelThreads < count) held[i0 + u * kSelThreads] = x[u];
+    }
+  };
+  if (!all && fits && n <= cap) hold_weights(0, n);
+  bad = __syncthreads_or(bad);
+  if (bad || all) {
+    for (uint32_t i = tid; i < e.keep; i += kSelThreads) {
+      kept[i] = !bad && i < n ? i : kNoSlot;
+      if (!bad && i < n && wo != w) wo[i] = w[i];
+    }
+    return;
+  }
+  const uint32_t old = n - e.recent, want = e.keep - e.recent;
+  // the sum of a and of b over the warps before this one, and over all (a, b: the same in all lanes)
+  auto scan = [&](uint32_t& a, uint32_t& b, uint32_t& all_a, uint32_t& all_b) {
+    if (lane == 0) {
+      warp_n[0][warp] = a;
+      warp_n[1][warp] = b;
+    }
     __syncthreads();
-    if (threadIdx.x < D) pool[to * D + threadIdx.x] = x;
-    if (threadIdx.x == 0 && !blockIdx.y) wo[i] = y;
+    const uint32_t x = warp_n[0][lane], y = warp_n[1][lane];
+    a = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+    b = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
+    all_a = __reduce_add_sync(0xffffffffu, x);
+    all_b = __reduce_add_sync(0xffffffffu, y);
+    __syncthreads();
+  };
+  uint32_t T = 0, left = want;  // the key's bits so far; how many of the keys that share them stay
+  for (int shift = 21; shift >= 0 && want; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
+    const uint32_t bits = shift ? 11 : 10;
+    for (uint32_t i = tid; i < kHists * kBins; i += kSelThreads) (&hist[0][0])[i] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = tid; i < old; i += kSelThreads) {
+      const uint32_t k = weight_key(fits ? held[i] : w[i]);
+      if (shift == 21 || (k ^ T) >> (shift + bits) == 0) atomicAdd(&hist[lane % kHists][k >> shift & ((1u << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // bins b, b - 1 (larger keys first: thread 0 has the last two)
+    const uint32_t b = kBins - 1 - 2 * tid;
+    uint32_t c1 = 0, c0 = 0;
+#pragma unroll
+    for (uint32_t v = 0; v < kHists; v++) {
+      c1 += hist[v][b];
+      c0 += hist[v][b - 1];
+    }
+    uint32_t sum = c1 + c0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    uint32_t before = __shfl_sync(0xffffffffu, sum, 31), none = 0, u0, u1;
+    scan(before, none, u0, u1);
+    const uint32_t above = before + sum - c1 - c0;  // keys in the bins before these two
+    if (above < left && above + c1 + c0 >= left) {
+      const bool second = above + c1 < left;
+      s_bin = b - second;
+      s_left = left - above - (second ? c1 : 0);
+    }
+    __syncthreads();
+    T |= s_bin << shift;
+    left = s_left;
+  }
+  uint32_t base = 0, ties = 0;  // kept so far; slots at T so far
+  for (uint32_t first = 0; first < n; first += hold) {
+    const uint32_t count = min(hold, n - first);
+    if (!fits) {
+      hold_weights(first, count);
+      __syncthreads();  // (read before any of these are written; what is written lies below all that is read later)
+    }
+    // a thread takes a run of slots (of an odd length: the threads then read from different banks)
+    const uint32_t run = (count + kSelThreads - 1) / kSelThreads | 1, r0 = min(count, tid * run), r1 = min(count, r0 + run);
+    auto above = [&](uint32_t i, uint32_t k) { return first + i >= old || (want && k > T); };
+    auto tie = [&](uint32_t i, uint32_t k) { return first + i < old && want && k == T; };
+    uint32_t a = 0, t = 0, all_a, all_t;
+    for (uint32_t i = r0; i < r1; i++) {
+      const uint32_t k = weight_key(held[i]);
+      a += above(i, k);
+      t += tie(i, k);
+    }
+    uint32_t sa = a, st = t;  // up to and with this thread, in the warp; then in the block, without it
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t ya = __shfl_up_sync(0xffffffffu, sa, o), yt = __shfl_up_sync(0xffffffffu, st, o);
+      if (lane >= o) {
+        sa += ya;
+        st += yt;
+      }
+    }
+    uint32_t wa = __shfl_sync(0xffffffffu, sa, 31), wt = __shfl_sync(0xffffffffu, st, 31);
+    scan(wa, wt, all_a, all_t);
+    const uint32_t ties_in = min(ties, left);
+    uint32_t ties_at = ties + wt + st - t, to = base + wa + sa - a + min(ties_at, left) - ties_in;
+    for (uint32_t i = r0; i < r1; i++) {
+      const uint32_t k = weight_key(held[i]);
+      const bool at_T = tie(i, k);
+      // (the ties that stay come among the others in slot order: as many before this one as fit)
+      if (above(i, k) || (at_T && ties_at < left)) {
+        kept[to] = first + i;
+        wo[to] = held[i];
+        to++;
+      }
+      ties_at += at_T;
+    }
+    base += all_a + min(ties + all_t, left) - ties_in;
+    ties += all_t;
     __syncthreads();
   }
-  if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) e.new_len[s] = m;
+}
+
+// Rows kept[i] of K or V to slot i, in 16-byte pieces: block (x: sequence and KV head; y:
+// K or V, and its share of a row's pieces; z: its share of the rows).  In place a sequence's rows move to
+// lower slots, kept[i] >= i ascending, so one block takes them all, tile by tile: a tile is written only
+// when the block has read it, and what it writes lies below all that later tiles read.  Elsewhere the tiles
+// are spread over the blocks.
+constexpr uint32_t kMoveThreads = 256, kMoveRows = 128;  // rows of a tile
+
+template <class T>
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move(PagedKV c, PagedEvict e, uint32_t shares) {
+  __shared__ uint32_t from_row[2][kMoveRows], to_row[2][kMoveRows];
+  const uint32_t s = blockIdx.x / c.kvheads, h = blockIdx.x % c.kvheads, tid = threadIdx.x;
+  const uint32_t share = blockIdx.y >> 1;
+  const uint32_t* const kept = e.kept + (uint64_t)blockIdx.x * e.keep;
+  const uint32_t n = e.len[s], m = min(n, e.keep);
+  // (new_len may be len: who reads it after this has the same m)
+  if (blockIdx.y == 0 && h == 0 && blockIdx.z == 0 && tid == 0) e.new_len[s] = kept[0] == kNoSlot ? n : m;
+  if (kept[0] == kNoSlot) return;  // nothing cached, or an invalid sequence
+  const uint32_t pieces = c.D * (uint32_t)sizeof(T) / 16, per = (pieces + shares - 1) / shares;
+  const uint32_t c0 = share * per, cn = min(pieces, c0 + per) - min(pieces, c0);
+  if (!cn) return;
+  uint8_t* const pool = static_cast<uint8_t*>(blockIdx.y & 1 ? c.v : c.k) + c0 * 16;
+  constexpr uint32_t kHold = 8;  // pieces a thread holds at once
+  const uint32_t step_row = kMoveThreads / cn, step_piece = kMoveThreads % cn;
+  uint32_t turn = 0;
+  for (uint32_t r0 = blockIdx.z * kMoveRows; r0 < m; r0 += gridDim.z * kMoveRows, turn ^= 1) {
+    const uint32_t rows = min(kMoveRows, m - r0);
+    if (tid < rows) {
+      from_row[turn][tid] = (uint32_t)pool_row(c, c.table, s, h, kept[r0 + tid]);
+      to_row[turn][tid] = (uint32_t)pool_row(c, e.dst_table, s, h, r0 + tid);
+    }
+    __syncthreads();
+    uint32_t row = tid / cn, piece = tid % cn;
+    for (uint32_t done = 0; done < rows * cn; done += kHold * kMoveThreads) {
+      uint4 x[kHold];
+      uint32_t row2 = row, piece2 = piece;
+      auto advance = [&](uint32_t& r, uint32_t& p) {
+        r += step_row;
+        p += step_piece;
+        if (p >= cn) {
+          p -= cn;
+          r++;
+        }
+      };
+#pragma unroll
+      for (uint32_t u = 0; u < kHold; u++) {
+        if (row < rows) x[u] = *reinterpret_cast<const uint4*>(pool + ((uint64_t)from_row[turn][row] * pieces + piece) * 16);
+        advance(row, piece);
+      }
+      __syncthreads();  // all of this part is read
+#pragma unroll
+      for (uint32_t u = 0; u < kHold; u++) {
+        if (row2 < rows) *reinterpret_cast<uint4*>(pool + ((uint64_t)to_row[turn][row2] * pieces + piece2) * 16) = x[u];
+        advance(row2, piece2);
+      }
+    }
+  }
 }
 
 }  // namespace
@@ -852,7 +971,7 @@ struct AttPrepare {
 
 // Once per device, before launch_paged_attention.
 cudaError_t paged_prepare() {
-  cudaError_t e = cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelHold * 4);
   for (uint32_t D : {32u, 64u, 96u, 128u, 192u, 256u}) {
     if (e == cudaSuccess) e = by_width<float>(D, AttPrepare{});
     if (e == cudaSuccess) e = by_width<__half>(D, AttPrepare{});
@@ -871,8 +990,17 @@ cudaError_t launch_paged_attention(const PagedKV& c, const PagedRows& r, cudaStr
 }
 
 cudaError_t launch_paged_evict(const PagedKV& c, const PagedEvict& e, cudaStream_t st) {
-  k_evict_select<<<c.n_seqs * c.kvheads, 1024, 0, st>>>(c, e);
-  QC_BY_KIND(c.kind, (k_evict_move<T><<<dim3(c.n_seqs * c.kvheads, 2), 256, 0, st>>>(c, e)));
+  const uint32_t units = c.n_seqs * c.kvheads, pieces = c.D * (c.kind == F32 ? 4 : 2) / 16;
+  const uint32_t cap = c.max_pages * c.page, hold = cap < kSelHold ? cap : kSelHold;
+  k_evict_select<<<units, kSelThreads, hold * 4, st>>>(c, e, hold);
+  // Enough blocks to fill the GPU, where there are few sequences: by rows, or in place by parts of a row
+  // (64 bytes at least).
+  uint32_t shares = 1, tiles = 1;
+  if (e.dst_table == c.table)
+    while ((uint64_t)units * 2 * shares < 1184 && pieces / (shares * 2) >= 4) shares *= 2;
+  else
+    while ((uint64_t)units * 2 * tiles < 2368 && tiles * kMoveRows < e.keep) tiles *= 2;
+  QC_BY_KIND(c.kind, (k_evict_move<T><<<dim3(units, 2 * shares, tiles), kMoveThreads, 0, st>>>(c, e, shares)));
   return cudaGetLastError();
 }
 
