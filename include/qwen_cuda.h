@@ -256,9 +256,10 @@ int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_page
  * A row of length 0 gives out 0 and lse -inf; so does one whose scores all overflow to -inf.  Slots a row
  * does not attend to may hold anything; a non-finite value among those it reads makes its results
  * non-finite.
- * weights (may be NULL): [n_seqs][kvheads][max_pages * page] f32; the softmax weights that the rows give
- * slot j, summed over a KV head's query heads, are added to weights[s][kv head][j], rows of one
- * sequence in call order.  The results do not depend on timing: the same call gives the same bits. */
+ * weights (may be NULL; needs lse, and with seq at most 131072 sequences): [n_seqs][kvheads][max_pages *
+ * page] f32; the softmax weights that the rows give slot j, summed over a KV head's query heads, are added
+ * to weights[s][kv head][j]; a head whose lse is NaN gives none.  The results do not depend on timing: the
+ * same call gives the same bits. */
 int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, uint32_t n_pages, uint32_t page,
                        uint32_t kvheads, uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages,
                        const float* q, uint32_t heads, uint32_t rows, const uint32_t* seq, const uint32_t* len, float scale,

@@ -2141,6 +2141,8 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     ensure(q && len && out, "null argument");
     ensure(seq || rows <= n_seqs, "more rows than sequences");
     ensure((uint64_t)rows * kvheads <= 0x7ffffffull, "too many rows");
+    ensure(!weights || lse, "weights need lse");
+    ensure(!weights || !seq || n_seqs <= qc::kMaxSharedSeqs, "weights with seq: more than 131072 sequences");
     DevicePointers at;
     at.add(k_pages, "k_pages", 16);
     at.add(v_pages, "v_pages", 16);
@@ -2152,7 +2154,8 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     at.add(lse, "lse");
     at.add(weights, "weights");
     at.enter();
-    qc::PagedRows r{q, heads, rows, seq, len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale, out, lse, weights};
+    qc::PagedRows r{q,   heads, rows,    seq,          len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale,
+                    out, lse,   weights, seq && rows > 1};
     QC_CK(qc::launch_paged_attention(c, r, static_cast<cudaStream_t>(stream)));
   });
 }

@@ -314,8 +314,10 @@ struct PagedRows {
   const uint32_t *seq, *len;
   float scale;
   float *out, *lse;  // [rows][heads][D], [rows][heads] or null
-  float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights
+  float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights (needs lse)
+  bool shared;       // with weights: several rows may name one sequence (n_seqs <= kMaxSharedSeqs)
 };
+constexpr uint32_t kMaxSharedSeqs = 1u << 17;
 constexpr uint32_t kNoSlot = 0xffffffffu;
 struct PagedEvict {
   const float* weights;

@@ -32,19 +32,42 @@ __device__ __forceinline__ uint64_t pool_row(const PagedKV& c, const uint32_t* t
   return ((uint64_t)p * c.kvheads + h) * c.page + j % c.page;
 }
 
-// Row i's k and v (f32, rounded to nearest) to slot pos[i] of sequence seq[i]; its weights become 0.
+// Eight values (four of f32) to nearest, as the 16 bytes of a cache row they make.
+template <class T>
+__device__ __forceinline__ uint4 round16(const float* x) {
+  const float4 a = *reinterpret_cast<const float4*>(x);
+  uint4 r;
+  if constexpr (sizeof(T) == 4) {
+    r = *reinterpret_cast<const uint4*>(&a);
+  } else {
+    const float4 b = *reinterpret_cast<const float4*>(x + 4);
+    const T v[8] = {from_float<T>(a.x), from_float<T>(a.y), from_float<T>(a.z), from_float<T>(a.w),
+                    from_float<T>(b.x), from_float<T>(b.y), from_float<T>(b.z), from_float<T>(b.w)};
+    memcpy(&r, v, 16);
+  }
+  return r;
+}
+
+// Row i's k and v (f32, rounded to nearest) to slot pos[i] of sequence seq[i]; its weights become 0.  A block
+// takes a row, a thread 16 bytes of the cache at a time, of k and of v.  A step's rows are bound by latency (the
+// row's place, then its values, then the write): 64 rows of 4 x 128 bf16 take 1.9 us; a prompt's by bytes:
+// 4500 rows of 8 x 128 f16 take 11.8 us, 4.7 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __restrict__ k, const float* __restrict__ v,
                                                        const uint32_t* __restrict__ seq, const uint32_t* __restrict__ pos,
                                                        float* __restrict__ weights) {
-  const uint32_t i = blockIdx.x, s = seq ? seq[i] : i, j = pos[i];
+  constexpr uint32_t kPer = 16 / sizeof(T);
+  const uint32_t i = blockIdx.x, s = seq ? seq[i] : i, j = pos[i], pieces = c.D / kPer;
   if (s >= c.n_seqs || j >= c.max_pages * c.page) return;
-  if (c.table[(uint64_t)s * c.max_pages + j / c.page] >= c.n_pages) return;
-  for (uint32_t e = threadIdx.x; e < c.kvheads * c.D; e += blockDim.x) {
-    const uint32_t h = e / c.D, d = e % c.D;
-    const uint64_t o = pool_row(c, c.table, s, h, j) * c.D + d, from = (uint64_t)i * c.kvheads * c.D + e;
-    static_cast<T*>(c.k)[o] = from_float<T>(k[from]);
-    static_cast<T*>(c.v)[o] = from_float<T>(v[from]);
+  const uint32_t at = j / c.page, in = j - at * c.page, p = c.table[(uint64_t)s * c.max_pages + at];
+  if (p >= c.n_pages) return;
+  for (uint32_t e = threadIdx.x; e < c.kvheads * pieces; e += blockDim.x) {
+    const uint32_t h = e / pieces;
+    const uint64_t to = (((uint64_t)p * c.kvheads + h) * c.page + in) * pieces + e % pieces;
+    const uint64_t from = ((uint64_t)i * c.kvheads * pieces + e) * kPer;
+    const uint4 a = round16<T>(k + from), b = round16<T>(v + from);
+    static_cast<uint4*>(c.k)[to] = a;
+    static_cast<uint4*>(c.v)[to] = b;
   }
   if (weights)
     for (uint32_t h = threadIdx.x; h < c.kvheads; h += blockDim.x)
@@ -85,8 +108,8 @@ struct Att {
   static constexpr int NS = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
   static constexpr int kRing = W * NS * kStage;
   static constexpr int kO = DP + 4;                                // floats between two heads' O in a warp's part
-  // ring; this block's share of every block's O; every block's 8 maxima, 8 sums and flag; the warps' maxima
-  static constexpr int kFixed = kRing + 8 * DP * 4 + kMaxCluster * 17 * 4 + W * 8 * 4;
+  // ring; this block's share of every block's O; every block's 8 maxima and 8 sums; the warps' maxima
+  static constexpr int kFixed = kRing + 8 * DP * 4 + kMaxCluster * 16 * 4 + W * 8 * 4;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -349,6 +372,9 @@ __device__ __forceinline__ void add_values(uint32_t vtile, const float (&p)[4], 
   }
 }
 
+// exp2(x - m) / l, with l's inverse; 0 where that is 0, whatever x.
+__device__ __forceinline__ float weight_of(float x, float m, float inv) { return inv == 0.f ? 0.f : pow2(x - m) * inv; }
+
 // How a launch splits a sequence: 2^logc blocks a cluster; a warp's next tile lies step_pages pages and
 // step_slots slots further; with weights, the tiles a warp keeps the scores of.
 struct AttSplit {
@@ -362,19 +388,20 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32, Att<T, DP>::kFixed <= 75 *
   constexpr int W = A::W, NS = A::NS;
   extern __shared__ __align__(16) uint8_t sm[];
   float* const in_o = reinterpret_cast<float*>(sm + A::kRing);  // [C][8 DP / C]: this block's share of every block's O
-  float* const in_m = in_o + 8 * DP;                            // [C][17]: every block's maxima, sums, flag
-  float* const warp_m = in_m + kMaxCluster * 17;                // [W][8]
-  const uint32_t C = 1u << sp.logc, rank = blockIdx.x & (C - 1), h = blockIdx.y, first = blockIdx.x >> sp.logc;
+  float* const in_m = in_o + 8 * DP;                            // [C][16]: every block's maxima, sums
+  float* const warp_m = in_m + kMaxCluster * 16;                // [W][8]
+  const uint32_t C = 1u << sp.logc, rank = blockIdx.x & (C - 1), h = blockIdx.y, i = blockIdx.x >> sp.logc;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
   uint8_t* const ring = sm + warp * NS * A::kStage;
   const uint32_t ring_a = smem_addr(ring);
-  const uint32_t s = r.seq ? r.seq[first] : first;
+  const uint32_t s = r.seq ? r.seq[i] : i, len = r.len[i];
   if (s >= c.n_seqs) return;  // (the whole cluster)
-  if (WEIGHTS && r.seq) {     // the cluster of a sequence's first row takes all its rows, in order
-    bool earlier = false;
-    for (uint32_t i = tid; i < first; i += W * 32) earlier |= r.seq[i] == s;
-    if (__syncthreads_or(earlier)) return;
+  bool give = WEIGHTS;  // (rows that share a sequence leave their weights to k_paged_weights)
+  if (WEIGHTS && r.shared) {
+    bool other = false;
+    for (uint32_t k = tid; k < r.rows; k += W * 32) other |= k != i && r.seq[k] == s;
+    give = !__syncthreads_or(other);
   }
   const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
   // Where pages hold whole runs of 8 positions (RUNS) a lane copies its part of a run with one address;
@@ -385,285 +412,428 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32, Att<T, DP>::kFixed <= 75 *
   const uint32_t page0 = (gw * kTile + ahead) / c.page, slot0 = (gw * kTile + ahead) % c.page;
   bool again = false;
 
-  for (uint32_t i = first; i < r.rows; i++) {
-    if (i > first && !(WEIGHTS && r.seq)) break;
-    if (i > first && r.seq[i] != s) continue;
-    const uint32_t len = r.len[i];
-    const bool too_long = len > cap;
-    const uint32_t tiles = too_long ? 0 : (len + kTile - 1) / kTile;
-    const uint32_t mine_n = tiles > gw ? (tiles - gw + C * W - 1) / (C * W) : 0;  // this warp's tiles
-    for (uint32_t g0 = 0; g0 < G; g0 += 8) {
-      const uint32_t gn = min(8u, G - g0);
-      bool bad = false;
-      Query<T, DP> q;
-      q.fetch(r.q + ((uint64_t)i * r.heads + h * G + g0) * D, D, gn);
-      auto clear_columns = [&](uint32_t rows) {  // columns D.. of the tiles are zero (the join writes over them)
-        const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
-        for (uint32_t e = lane; e < rows * extra; e += 32)
-          *reinterpret_cast<uint4*>(ring + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
-      };
-      // The page number of position j, table entry `at`, and its row at slot `in` for the tile from j0 on.
-      auto page_at = [&](uint32_t j, uint32_t at) { return j < len && !too_long ? pages[at] : kNoSlot; };
-      auto row_of = [&](uint32_t p, uint32_t in, uint32_t j0) {
-        if (p >= c.n_pages) {
-          bad |= j0 + ahead < len;
-          return kNoSlot;
-        }
-        return (p * c.kvheads + h) * c.page + in;
-      };
-      // Copies the tile of positions j0.. into a ring slot; row: this lane's lookup.
-      auto fetch = [&](uint32_t slot, uint32_t row, uint32_t j0, bool with_v) {
-        constexpr uint32_t kCh = DP * sizeof(T) / 16;
-        const uint32_t dst = ring_a + slot * A::kStage;
-        const uint8_t *kp = static_cast<const uint8_t*>(c.k), *vp = static_cast<const uint8_t*>(c.v);
-        if (runs) {
-          const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0), row1 = __shfl_sync(0xffffffffu, row, 16);
-          const uint64_t bytes = D * sizeof(T);
-          const uint64_t at0 = row0 == kNoSlot ? 0 : row0 * bytes, at1 = (row1 == kNoSlot ? 0 : row1 * bytes) - 8 * bytes;
-          const uint32_t n = j0 < len ? len - j0 : 0, n0 = row0 == kNoSlot ? 0 : n, n1 = row1 == kNoSlot ? 0 : n;
+  const bool too_long = len > cap;
+  const uint32_t tiles = too_long ? 0 : (len + kTile - 1) / kTile;
+  const uint32_t mine_n = tiles > gw ? (tiles - gw + C * W - 1) / (C * W) : 0;  // this warp's tiles
+  for (uint32_t g0 = 0; g0 < G; g0 += 8) {
+    const uint32_t gn = min(8u, G - g0);
+    bool bad = false;
+    Query<T, DP> q;
+    q.fetch(r.q + ((uint64_t)i * r.heads + h * G + g0) * D, D, gn);
+    auto clear_columns = [&](uint32_t rows) {  // columns D.. of the tiles are zero (the join writes over them)
+      const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
+      for (uint32_t e = lane; e < rows * extra; e += 32)
+        *reinterpret_cast<uint4*>(ring + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
+    };
+    // The page number of position j, table entry `at`, and its row at slot `in` for the tile from j0 on.
+    auto page_at = [&](uint32_t j, uint32_t at) { return j < len && !too_long ? pages[at] : kNoSlot; };
+    auto row_of = [&](uint32_t p, uint32_t in, uint32_t j0) {
+      if (p >= c.n_pages) {
+        bad |= j0 + ahead < len;
+        return kNoSlot;
+      }
+      return (p * c.kvheads + h) * c.page + in;
+    };
+    // Copies the tile of positions j0.. into a ring slot; row: this lane's lookup.
+    auto fetch = [&](uint32_t slot, uint32_t row, uint32_t j0, bool with_v) {
+      constexpr uint32_t kCh = DP * sizeof(T) / 16;
+      const uint32_t dst = ring_a + slot * A::kStage;
+      const uint8_t *kp = static_cast<const uint8_t*>(c.k), *vp = static_cast<const uint8_t*>(c.v);
+      if (runs) {
+        const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0), row1 = __shfl_sync(0xffffffffu, row, 16);
+        const uint64_t bytes = D * sizeof(T);
+        const uint64_t at0 = row0 == kNoSlot ? 0 : row0 * bytes, at1 = (row1 == kNoSlot ? 0 : row1 * bytes) - 8 * bytes;
+        const uint32_t n = j0 < len ? len - j0 : 0, n0 = row0 == kNoSlot ? 0 : n, n1 = row1 == kNoSlot ? 0 : n;
 #pragma unroll
-          for (uint32_t e0 = 0; e0 < kTile * kCh; e0 += 32) {
-            const uint32_t e = e0 + lane, p = e / kCh, ch = e % kCh;
-            const bool second = e0 >= 8 * kCh;
-            const uint64_t o = (second ? at1 : at0) + (p * chunks + ch) * 16;
-            const bool real = p < (second ? n1 : n0);
-            if (DP * sizeof(T) != chunks * 16 && ch >= chunks) continue;
-            copy16(dst + p * A::kRow + ch * 16, kp + o, real);
-            if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, real);
-          }
-        } else {
+        for (uint32_t e0 = 0; e0 < kTile * kCh; e0 += 32) {
+          const uint32_t e = e0 + lane, p = e / kCh, ch = e % kCh;
+          const bool second = e0 >= 8 * kCh;
+          const uint64_t o = (second ? at1 : at0) + (p * chunks + ch) * 16;
+          const bool real = p < (second ? n1 : n0);
+          if (DP * sizeof(T) != chunks * 16 && ch >= chunks) continue;
+          copy16(dst + p * A::kRow + ch * 16, kp + o, real);
+          if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, real);
+        }
+      } else {
 #pragma unroll 4
-          for (uint32_t e = lane; e < kTile * kCh; e += 32) {
-            const uint32_t p = e / kCh, ch = e % kCh;
-            const uint32_t from = __shfl_sync(0xffffffffu, row, p);
-            const uint64_t o = from == kNoSlot ? 0 : (uint64_t)from * D * sizeof(T) + ch * 16;
-            if (ch >= chunks) continue;
-            copy16(dst + p * A::kRow + ch * 16, kp + o, from != kNoSlot);
-            if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, from != kNoSlot);
-          }
+        for (uint32_t e = lane; e < kTile * kCh; e += 32) {
+          const uint32_t p = e / kCh, ch = e % kCh;
+          const uint32_t from = __shfl_sync(0xffffffffu, row, p);
+          const uint64_t o = from == kNoSlot ? 0 : (uint64_t)from * D * sizeof(T) + ch * 16;
+          if (ch >= chunks) continue;
+          copy16(dst + p * A::kRow + ch * 16, kp + o, from != kNoSlot);
+          if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, from != kNoSlot);
         }
-      };
-      // this warp's tiles one after the other
-      uint32_t j = gw * kTile + ahead, at = page0, in = slot0;
-      auto advance = [&] {
-        j += step;
-        at += sp.step_pages;
-        in += sp.step_slots;
-        if (in >= c.page) {
-          in -= c.page;
-          at++;
+      }
+    };
+    // this warp's tiles one after the other
+    uint32_t j = gw * kTile + ahead, at = page0, in = slot0;
+    auto advance = [&] {
+      j += step;
+      at += sp.step_pages;
+      in += sp.step_slots;
+      if (in >= c.page) {
+        in -= c.page;
+        at++;
+      }
+    };
+    uint32_t pg[NS], slots[NS];
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+      pg[n] = page_at(j, at);
+      slots[n] = in;
+      advance();
+    }
+    uint32_t next = page_at(j, at), next_in = in, j0 = gw * kTile;
+    if (chunks * 16 < DP * sizeof(T)) clear_columns(2 * NS * kTile);
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+      fetch(n, row_of(pg[n], slots[n], j0), j0, true);
+      copy_commit();
+      j0 += step;
+    }
+    q.split(r.scale * 1.4426950408889634f);
+    float o[DP / 16][4], m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
+    float4* const kept_scores = reinterpret_cast<float4*>(sm + A::kFixed) + (uint64_t)warp * sp.score_tiles * 32 + lane;
+    auto masked_scores = [&](uint32_t n, uint32_t ktile, float (&x)[4]) {
+      q.scores(ktile, x);
+      const uint32_t pos = gw * kTile + n * step + g;
+      if (pos >= len) x[0] = x[1] = -INFINITY;
+      if (pos + 8 >= len) x[2] = x[3] = -INFINITY;
+    };
+    for (uint32_t n = 0, slot = 0; n < mine_n; n++, slot = slot + 1 == NS ? 0 : slot + 1) {
+      copy_wait<NS - 1>();
+      __syncwarp();
+      const uint32_t tile_a = ring_a + slot * A::kStage;
+      float x[4];
+      masked_scores(n, tile_a, x);
+      if (WEIGHTS && give && n < sp.score_tiles) kept_scores[n * 32] = make_float4(x[0], x[1], x[2], x[3]);
+      const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
+      if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
+        float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
+#pragma unroll
+        for (int w = 4; w < 32; w *= 2) {
+          n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
         }
-      };
-      uint32_t pg[NS], slots[NS];
+        const float f0 = pow2(m0 - n0), f1 = pow2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
 #pragma unroll
-      for (int n = 0; n < NS; n++) {
-        pg[n] = page_at(j, at);
-        slots[n] = in;
-        advance();
+        for (auto& y : o) {
+          y[0] *= f0;
+          y[1] *= f1;
+          y[2] *= f0;
+          y[3] *= f1;
+        }
       }
-      uint32_t next = page_at(j, at), next_in = in, j0 = gw * kTile;
-      if (chunks * 16 < DP * sizeof(T)) clear_columns(2 * NS * kTile);
+      const float p[4] = {pow2(x[0] - m0), pow2(x[1] - m1), pow2(x[2] - m0), pow2(x[3] - m1)};
+      l0 += p[0] + p[2];
+      l1 += p[1] + p[3];
+      add_values<T, DP>(tile_a + kTile * A::kRow, p, o);
+      __syncwarp();
+      fetch(slot, row_of(next, next_in, j0), j0, true);
+      copy_commit();
+      j0 += step;
+      advance();
+      next = page_at(j, at);
+      next_in = in;
+    }
+    copy_wait<0>();
+    // the warps of the block: O and sums relative to the block's maxima, then added up
 #pragma unroll
-      for (int n = 0; n < NS; n++) {
-        fetch(n, row_of(pg[n], slots[n], j0), j0, true);
-        copy_commit();
-        j0 += step;
+    for (int w = 4; w < 32; w *= 2) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, w);
+    }
+    if (g == 0) {
+      warp_m[warp * 8 + 2 * t] = m0;
+      warp_m[warp * 8 + 2 * t + 1] = m1;
+    }
+    bad = __syncthreads_or(bad) || too_long;
+    float M0 = m0, M1 = m1;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      M0 = fmaxf(M0, warp_m[w * 8 + 2 * t]);
+      M1 = fmaxf(M1, warp_m[w * 8 + 2 * t + 1]);
+    }
+    const float f0 = pow2(m0 - M0), f1 = pow2(m1 - M1);
+    float* const mine = reinterpret_cast<float*>(ring);  // [8][kO], sums
+#pragma unroll
+    for (int m = 0; m < DP / 16; m++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        mine[(2 * t + e % 2) * A::kO + m * 16 + g + (e / 2) * 8] = o[m][e] * (e % 2 ? f1 : f0);
+    if (g == 0) {
+      mine[8 * A::kO + 2 * t] = l0 * f0;
+      mine[8 * A::kO + 2 * t + 1] = l1 * f1;
+    }
+    if (again) cluster_sync();  // the other blocks have read what was sent for the previous turn
+    else __syncthreads();
+    again = true;
+    // what they add up to goes to the blocks of the cluster: a share of O to each, maxima and sums to all
+    auto part = [&](uint32_t w) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage); };
+    const uint32_t share = (2 * DP) >> sp.logc;  // 16-byte pieces of O of one block
+    for (uint32_t e = tid; e < 2 * DP; e += W * 32) {
+      const uint32_t hh = e / (DP / 4), d = e % (DP / 4) * 4;
+      float4 sum = *reinterpret_cast<const float4*>(part(0) + hh * A::kO + d);
+#pragma unroll
+      for (int w = 1; w < W; w++) {
+        const float4 y = *reinterpret_cast<const float4*>(part(w) + hh * A::kO + d);
+        sum.x += y.x;
+        sum.y += y.y;
+        sum.z += y.z;
+        sum.w += y.w;
       }
-      q.split(r.scale * 1.4426950408889634f);
-      float o[DP / 16][4], m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
+      const uint32_t to = e / share;
+      st_cluster4(cluster_addr(smem_addr(in_o) + (rank * share + e - to * share) * 16, to), sum);
+    }
+    for (uint32_t e = tid; e < C * 8; e += W * 32) {
+      const uint32_t hh = e % 8, to = e / 8;
+      float M = warp_m[hh], L = part(0)[8 * A::kO + hh];
 #pragma unroll
-      for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
-      float4* const kept_scores = reinterpret_cast<float4*>(sm + A::kFixed) + (uint64_t)warp * sp.score_tiles * 32 + lane;
-      auto masked_scores = [&](uint32_t n, uint32_t ktile, float (&x)[4]) {
-        q.scores(ktile, x);
-        const uint32_t pos = gw * kTile + n * step + g;
-        if (pos >= len) x[0] = x[1] = -INFINITY;
-        if (pos + 8 >= len) x[2] = x[3] = -INFINITY;
-      };
-      for (uint32_t n = 0, slot = 0; n < mine_n; n++, slot = slot + 1 == NS ? 0 : slot + 1) {
-        copy_wait<NS - 1>();
+      for (int w = 1; w < W; w++) {
+        M = fmaxf(M, warp_m[w * 8 + hh]);
+        L += part(w)[8 * A::kO + hh];
+      }
+      const uint32_t a = cluster_addr(smem_addr(in_m) + rank * 16 * 4, to);
+      st_cluster(a + hh * 4, M);
+      st_cluster(a + 32 + hh * 4, bad ? __int_as_float(0x7fc00000) : L);
+    }
+    cluster_sync();
+    // the maximum and the sum of head hh over the blocks (bad: NaN)
+    auto total = [&](uint32_t hh, float& M, float& L) {
+      M = -FLT_MAX;
+      L = 0.f;
+#pragma unroll 4
+      for (uint32_t k = 0; k < C; k++) M = fmaxf(M, in_m[k * 16 + hh]);
+#pragma unroll 4
+      for (uint32_t k = 0; k < C; k++) L = fmaf(in_m[k * 16 + 8 + hh], pow2(in_m[k * 16 + hh] - M), L);
+    };
+    const uint64_t row_head = (uint64_t)i * r.heads + h * G + g0;
+    for (uint32_t e = tid; e < share; e += W * 32) {
+      const uint32_t hh = (rank * share + e) / (DP / 4), d = (rank * share + e) % (DP / 4) * 4;
+      if (hh >= gn || d >= D) continue;
+      float M, L;
+      total(hh, M, L);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (uint32_t k = 0; k < C; k++) {
+        const float f = pow2(in_m[k * 16 + hh] - M);
+        const float4 y = reinterpret_cast<const float4*>(in_o)[k * share + e];
+        sum.x = fmaf(y.x, f, sum.x);
+        sum.y = fmaf(y.y, f, sum.y);
+        sum.z = fmaf(y.z, f, sum.z);
+        sum.w = fmaf(y.w, f, sum.w);
+      }
+      const float inv = L == 0.f ? 0.f : (__is_same(T, __half) ? 1.f / 16384.f : 1.f) / L;
+      *reinterpret_cast<float4*>(r.out + (row_head + hh) * D + d) =
+          make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+      if (d == 0 && r.lse) r.lse[row_head + hh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    }
+    if (WEIGHTS && give) {
+      float M[2], inv[2];  // (a head whose sum is NaN, as where a page is bad, gives no weights)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float L;
+        total(2 * t + u, M[u], L);
+        inv[u] = 2 * t + u >= gn || !(L > 0.f) ? 0.f : 1.f / L;
+      }
+      if (mine_n > sp.score_tiles && chunks * 16 < DP * sizeof(T)) {
         __syncwarp();
-        const uint32_t tile_a = ring_a + slot * A::kStage;
-        float x[4];
-        masked_scores(n, tile_a, x);
-        if (WEIGHTS && n < sp.score_tiles) kept_scores[n * 32] = make_float4(x[0], x[1], x[2], x[3]);
-        const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
-        if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
-          float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
+        clear_columns(kTile);
+      }
+      float* const w = r.weights + ((uint64_t)s * c.kvheads + h) * cap;
+      // (the weights' reads first, four tiles at a time: one after the other each would wait for the last)
+      for (uint32_t n0 = 0; n0 < mine_n; n0 += 4) {
+        float old[4];
 #pragma unroll
-          for (int w = 4; w < 32; w *= 2) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
+        for (uint32_t u = 0; u < 4; u++) {
+          const uint32_t pos = gw * kTile + (n0 + u) * step + g + 8 * t;
+          old[u] = t < 2 && n0 + u < mine_n && pos < len ? w[pos] : 0.f;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++) {
+          const uint32_t n = n0 + u, base = gw * kTile + n * step, pos = base + ahead;
+          if (n >= mine_n) break;
+          float x[4];
+          if (n < sp.score_tiles) {
+            const float4 y = kept_scores[n * 32];
+            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+          } else {
+            __syncwarp();
+            fetch(0, row_of(page_at(pos, pos / c.page), pos % c.page, base), base, false);
+            copy_commit();
+            copy_wait<0>();
+            __syncwarp();
+            masked_scores(n, ring_a, x);
           }
-          const float f0 = pow2(m0 - n0), f1 = pow2(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          l0 *= f0;
-          l1 *= f1;
-#pragma unroll
-          for (auto& y : o) {
-            y[0] *= f0;
-            y[1] *= f1;
-            y[2] *= f0;
-            y[3] *= f1;
-          }
-        }
-        const float p[4] = {pow2(x[0] - m0), pow2(x[1] - m1), pow2(x[2] - m0), pow2(x[3] - m1)};
-        l0 += p[0] + p[2];
-        l1 += p[1] + p[3];
-        add_values<T, DP>(tile_a + kTile * A::kRow, p, o);
-        __syncwarp();
-        fetch(slot, row_of(next, next_in, j0), j0, true);
-        copy_commit();
-        j0 += step;
-        advance();
-        next = page_at(j, at);
-        next_in = in;
-      }
-      copy_wait<0>();
-      // the warps of the block: O and sums relative to the block's maxima, then added up
-#pragma unroll
-      for (int w = 4; w < 32; w *= 2) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, w);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, w);
-      }
-      if (g == 0) {
-        warp_m[warp * 8 + 2 * t] = m0;
-        warp_m[warp * 8 + 2 * t + 1] = m1;
-      }
-      bad = __syncthreads_or(bad) || too_long;
-      float M0 = m0, M1 = m1;
-#pragma unroll
-      for (int w = 0; w < W; w++) {
-        M0 = fmaxf(M0, warp_m[w * 8 + 2 * t]);
-        M1 = fmaxf(M1, warp_m[w * 8 + 2 * t + 1]);
-      }
-      const float f0 = pow2(m0 - M0), f1 = pow2(m1 - M1);
-      float* const mine = reinterpret_cast<float*>(ring);  // [8][kO], sums
-#pragma unroll
-      for (int m = 0; m < DP / 16; m++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          mine[(2 * t + e % 2) * A::kO + m * 16 + g + (e / 2) * 8] = o[m][e] * (e % 2 ? f1 : f0);
-      if (g == 0) {
-        mine[8 * A::kO + 2 * t] = l0 * f0;
-        mine[8 * A::kO + 2 * t + 1] = l1 * f1;
-      }
-      if (again) cluster_sync();  // the other blocks have read what was sent for the previous turn
-      else __syncthreads();
-      again = true;
-      // what they add up to goes to the blocks of the cluster: a share of O to each, maxima and sums to all
-      auto part = [&](uint32_t w) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage); };
-      const uint32_t share = (2 * DP) >> sp.logc;  // 16-byte pieces of O of one block
-      for (uint32_t e = tid; e < 2 * DP; e += W * 32) {
-        const uint32_t hh = e / (DP / 4), d = e % (DP / 4) * 4;
-        float4 sum = *reinterpret_cast<const float4*>(part(0) + hh * A::kO + d);
-#pragma unroll
-        for (int w = 1; w < W; w++) {
-          const float4 y = *reinterpret_cast<const float4*>(part(w) + hh * A::kO + d);
-          sum.x += y.x;
-          sum.y += y.y;
-          sum.z += y.z;
-          sum.w += y.w;
-        }
-        const uint32_t to = e / share;
-        st_cluster4(cluster_addr(smem_addr(in_o) + (rank * share + e - to * share) * 16, to), sum);
-      }
-      for (uint32_t e = tid; e < C * 8; e += W * 32) {
-        const uint32_t hh = e % 8, to = e / 8;
-        float M = warp_m[hh], L = part(0)[8 * A::kO + hh];
-#pragma unroll
-        for (int w = 1; w < W; w++) {
-          M = fmaxf(M, warp_m[w * 8 + hh]);
-          L += part(w)[8 * A::kO + hh];
-        }
-        const uint32_t a = cluster_addr(smem_addr(in_m) + rank * 17 * 4, to);
-        st_cluster(a + hh * 4, M);
-        st_cluster(a + 32 + hh * 4, bad ? __int_as_float(0x7fc00000) : L);
-        if (hh == 0) st_cluster(a + 64, bad ? 1.f : 0.f);
-      }
-      cluster_sync();
-      // the maximum and the sum of head hh over the blocks (bad: NaN)
-      auto total = [&](uint32_t hh, float& M, float& L) {
-        M = -FLT_MAX;
-        L = 0.f;
-#pragma unroll 4
-        for (uint32_t k = 0; k < C; k++) M = fmaxf(M, in_m[k * 17 + hh]);
-#pragma unroll 4
-        for (uint32_t k = 0; k < C; k++) L = fmaf(in_m[k * 17 + 8 + hh], pow2(in_m[k * 17 + hh] - M), L);
-      };
-      const uint64_t row_head = (uint64_t)i * r.heads + h * G + g0;
-      for (uint32_t e = tid; e < share; e += W * 32) {
-        const uint32_t hh = (rank * share + e) / (DP / 4), d = (rank * share + e) % (DP / 4) * 4;
-        if (hh >= gn || d >= D) continue;
-        float M, L;
-        total(hh, M, L);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (uint32_t k = 0; k < C; k++) {
-          const float f = pow2(in_m[k * 17 + hh] - M);
-          const float4 y = reinterpret_cast<const float4*>(in_o)[k * share + e];
-          sum.x = fmaf(y.x, f, sum.x);
-          sum.y = fmaf(y.y, f, sum.y);
-          sum.z = fmaf(y.z, f, sum.z);
-          sum.w = fmaf(y.w, f, sum.w);
-        }
-        const float inv = L == 0.f ? 0.f : (__is_same(T, __half) ? 1.f / 16384.f : 1.f) / L;
-        *reinterpret_cast<float4*>(r.out + (row_head + hh) * D + d) =
-            make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-        if (d == 0 && r.lse) r.lse[row_head + hh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-      }
-      if (WEIGHTS) {
-        bad = false;
-        for (uint32_t k = 0; k < C; k++) bad |= in_m[k * 17 + 16] != 0.f;
-        float M[2], inv[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          float L;
-          total(2 * t + u, M[u], L);
-          inv[u] = 2 * t + u >= gn || L == 0.f ? 0.f : 1.f / L;
-        }
-        if (mine_n > sp.score_tiles && chunks * 16 < DP * sizeof(T)) {
-          __syncwarp();
-          clear_columns(kTile);
-        }
-        float* const w = r.weights + ((uint64_t)s * c.kvheads + h) * cap;
-        // (the weights' reads first, four tiles at a time: one after the other each would wait for the last)
-        for (uint32_t n0 = 0; n0 < mine_n && !bad; n0 += 4) {
-          float old[4];
-#pragma unroll
-          for (uint32_t u = 0; u < 4; u++) {
-            const uint32_t pos = gw * kTile + (n0 + u) * step + g + 8 * t;
-            old[u] = t < 2 && n0 + u < mine_n && pos < len ? w[pos] : 0.f;
-          }
-#pragma unroll
-          for (uint32_t u = 0; u < 4; u++) {
-            const uint32_t n = n0 + u, base = gw * kTile + n * step, pos = base + ahead;
-            if (n >= mine_n) break;
-            float x[4];
-            if (n < sp.score_tiles) {
-              const float4 y = kept_scores[n * 32];
-              x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-            } else {
-              __syncwarp();
-              fetch(0, row_of(page_at(pos, pos / c.page), pos % c.page, base), base, false);
-              copy_commit();
-              copy_wait<0>();
-              __syncwarp();
-              masked_scores(n, ring_a, x);
-            }
-            float w0 = pow2(x[0] - M[0]) * inv[0] + pow2(x[1] - M[1]) * inv[1];
-            float w8 = pow2(x[2] - M[0]) * inv[0] + pow2(x[3] - M[1]) * inv[1];
-            w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
-            w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
-            w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
-            w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
-            if (t < 2 && base + g + 8 * t < len) w[base + g + 8 * t] = old[u] + (t ? w8 : w0);
-          }
+          float w0 = weight_of(x[0], M[0], inv[0]) + weight_of(x[1], M[1], inv[1]);
+          float w8 = weight_of(x[2], M[0], inv[0]) + weight_of(x[3], M[1], inv[1]);
+          w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+          w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
+          w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+          w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
+          if (t < 2 && base + g + 8 * t < len) w[base + g + 8 * t] = old[u] + (t ? w8 : w0);
         }
       }
     }
   }
+}
+
+// Weights of rows that share a sequence (a prompt's tokens): the attention above leaves them out, as its
+// clusters would have to add to the same slots one after the other.  Here a warp takes a tile of 16
+// positions and goes through its sequence's rows in call order: scores again (K is read once more for all
+// rows together), weights exp(s - lse) from the rows' lse, summed over heads and rows in registers, one
+// addition to the slot at the end.  The rows' operands are split into planes once a block, a row a warp.
+// A launch has two blocks an SM; each finds the sequences that two rows or more name, in one pass over
+// seq, and ends at once when there are none.
+template <class T, int DP>
+struct Give {
+  using A = Att<T, DP>;
+  static constexpr int kTileBytes = kTile * A::kRow;
+  static constexpr int kWords = (A::kKS * A::kQP * 2 + 2 + 3) / 4 * 4;  // of a row's operand, a lane
+  static constexpr int W = 8 * (kTileBytes + kWords * 128) <= 104 * 1024 ? 8 : 4;
+  static constexpr int kList = W * 32;                                  // rows at a time
+  static constexpr int kSmem = W * (kTileBytes + kWords * 128) + W * 48 + kList * 4 + 64;  // and two bits a sequence
+};
+
+template <class T, int DP>
+__global__ void __launch_bounds__(Give<T, DP>::W * 32) k_paged_weights(PagedKV c, PagedRows r) {
+  using A = Att<T, DP>;
+  using B = Give<T, DP>;
+  constexpr int W = B::W;
+  extern __shared__ __align__(16) uint8_t sm[];
+  uint4* const operands = reinterpret_cast<uint4*>(sm + W * B::kTileBytes);        // [W rows][kWords / 4][32 lanes]
+  float* const row_lse = reinterpret_cast<float*>(operands + W * B::kWords * 8);   // [W][8], times log2 e; inf: no weights
+  uint32_t* const row_len = reinterpret_cast<uint32_t*>(row_lse + W * 8);          // [W]
+  uint32_t* const list = row_len + W * 4;                                          // [kList]
+  uint32_t* const warp_n = list + B::kList;                                        // [W], at most 16
+  uint32_t* const seen = warp_n + 16;
+  const uint32_t words = (c.n_seqs + 31) / 32;
+  uint32_t* const twice = seen + words;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
+  const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
+  for (uint32_t k = tid; k < 2 * words; k += W * 32) seen[k] = 0;
+  __syncthreads();
+  for (uint32_t k = tid; k < r.rows; k += W * 32) {
+    const uint32_t s = r.seq[k];
+    if (s < c.n_seqs && atomicOr(&seen[s / 32], 1u << s % 32) >> s % 32 & 1) atomicOr(&twice[s / 32], 1u << s % 32);
+  }
+  __syncthreads();
+  uint8_t* const tile = sm + warp * B::kTileBytes;
+  const uint32_t tile_a = smem_addr(tile);
+  if (chunks * 16 < DP * sizeof(T)) {
+    const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
+    for (uint32_t e = lane; e < kTile * extra; e += 32)
+      *reinterpret_cast<uint4*>(tile + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  for (uint32_t word = 0; word < words; word++)
+    for (uint32_t bits = twice[word]; bits; bits &= bits - 1) {
+      const uint32_t s = word * 32 + __ffs(bits) - 1;
+      const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
+      uint32_t longest = 0;  // (rows longer than the cache give no weights)
+      for (uint32_t k = tid; k < r.rows; k += W * 32)
+        if (r.seq[k] == s && r.len[k] <= cap) longest = max(longest, r.len[k]);
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      __syncthreads();
+      if (lane == 0) warp_n[warp] = longest;
+      __syncthreads();
+      for (uint32_t v = 0; v < W; v++) longest = max(longest, warp_n[v]);
+      const uint32_t blocks = (longest + W * kTile - 1) / (W * kTile);
+      for (uint32_t from = 0; from < r.rows; from += B::kList) {  // (the same warp takes a tile every time)
+        const uint32_t k = from + tid;
+        const bool is = k < r.rows && r.seq[k] == s;
+        const uint32_t who = __ballot_sync(0xffffffffu, is);
+        __syncthreads();
+        if (lane == 0) warp_n[warp] = __popc(who);
+        __syncthreads();
+        uint32_t at = 0, n = 0;
+        for (uint32_t v = 0; v < W; v++) {
+          if (v == warp) at = n;
+          n += warp_n[v];
+        }
+        if (is) list[at + __popc(who & ((1u << lane) - 1))] = k;
+        __syncthreads();
+        for (uint32_t item = n ? blockIdx.x : 0xffffffffu; item < blocks * c.kvheads; item += gridDim.x) {
+          const uint32_t h = item / blocks, j0 = (item % blocks * W + warp) * kTile;
+          const uint32_t j = j0 + lane % kTile, p = j < longest ? pages[j / c.page] : kNoSlot;
+          const uint32_t row = p < c.n_pages ? (p * c.kvheads + h) * c.page + j % c.page : kNoSlot;
+          constexpr uint32_t kCh = DP * sizeof(T) / 16;
+          for (uint32_t e = lane; e < kTile * kCh; e += 32) {
+            const uint32_t pos = e / kCh, ch = e % kCh, src = __shfl_sync(0xffffffffu, row, pos);
+            if (ch < chunks)
+              copy16(tile_a + pos * A::kRow + ch * 16,
+                     static_cast<const uint8_t*>(c.k) + (src == kNoSlot ? 0 : (uint64_t)src * D * sizeof(T) + ch * 16),
+                     src != kNoSlot);
+          }
+          copy_commit();
+          float w0 = 0.f, w8 = 0.f;  // of positions j0 + g and j0 + g + 8, this lane's heads
+          for (uint32_t g0 = 0; g0 < G; g0 += 8)
+            for (uint32_t k0 = 0; k0 < n; k0 += W) {
+              __syncthreads();  // the operands before are done with
+              Query<T, DP> q;
+              if (k0 + warp < n) {
+                const uint32_t i = list[k0 + warp], gn = min(8u, G - g0);
+                const uint64_t head = (uint64_t)i * r.heads + h * G + g0;
+                q.fetch(r.q + head * D, D, gn);
+                q.split(r.scale * 1.4426950408889634f);
+                uint32_t v[B::kWords] = {};
+#pragma unroll
+                for (int e = 0; e < A::kKS * A::kQP * 2; e++) v[e] = q.f[e / (A::kQP * 2)][e / 2 % A::kQP][e % 2];
+                v[A::kKS * A::kQP * 2] = __float_as_uint(q.undo0);
+                v[A::kKS * A::kQP * 2 + 1] = __float_as_uint(q.undo1);
+#pragma unroll
+                for (int e = 0; e < B::kWords / 4; e++)
+                  operands[(warp * (B::kWords / 4) + e) * 32 + lane] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                if (lane < 8) {
+                  const float lse = lane < gn ? r.lse[head + lane] : INFINITY;
+                  row_lse[warp * 8 + lane] = fabsf(lse) < INFINITY ? lse * 1.4426950408889634f : INFINITY;
+                }
+                if (lane == 0) row_len[warp] = r.len[i] <= cap ? r.len[i] : 0;
+              }
+              copy_wait<0>();
+              __syncthreads();
+              for (uint32_t k1 = 0; k1 < min((uint32_t)W, n - k0); k1++) {
+                const uint32_t len = row_len[k1];
+                if (j0 >= len) continue;
+                uint32_t v[B::kWords];
+#pragma unroll
+                for (int e = 0; e < B::kWords / 4; e++)
+                  *reinterpret_cast<uint4*>(v + 4 * e) = operands[(k1 * (B::kWords / 4) + e) * 32 + lane];
+#pragma unroll
+                for (int e = 0; e < A::kKS * A::kQP * 2; e++) q.f[e / (A::kQP * 2)][e / 2 % A::kQP][e % 2] = v[e];
+                q.undo0 = __uint_as_float(v[A::kKS * A::kQP * 2]);
+                q.undo1 = __uint_as_float(v[A::kKS * A::kQP * 2 + 1]);
+                float x[4];
+                q.scores(tile_a, x);
+                const float lse0 = row_lse[k1 * 8 + 2 * t], lse1 = row_lse[k1 * 8 + 2 * t + 1];
+                const bool in0 = j0 + g < len, in8 = j0 + g + 8 < len;
+                if (lse0 < INFINITY) {
+                  w0 += in0 ? pow2(x[0] - lse0) : 0.f;
+                  w8 += in8 ? pow2(x[2] - lse0) : 0.f;
+                }
+                if (lse1 < INFINITY) {
+                  w0 += in0 ? pow2(x[1] - lse1) : 0.f;
+                  w8 += in8 ? pow2(x[3] - lse1) : 0.f;
+                }
+              }
+            }
+          w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+          w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
+          w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+          w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
+          const uint32_t slot = j0 + g + 8 * t;
+          if (t < 2 && slot < longest) r.weights[((uint64_t)s * c.kvheads + h) * cap + slot] += t ? w8 : w0;
+          __syncwarp();  // (the tile is read)
+        }
+        __syncthreads();
+      }
+    }
 }
 
 // A weight's place in the order of eviction: larger weights have larger keys, NaN the smallest.
@@ -683,8 +853,8 @@ constexpr uint32_t kHists = 4, kBins = 2048;
 // The want-th largest key is found by its first 11, next 11 and last 10 bits: a histogram of the keys that
 // share the bits found so far (four, for every fourth lane: the first bits bunch up), then a scan over its
 // bins.  Then the slots above it and the first ones at it are numbered: each thread counts its run of
-// slots, and knows its place from the counts of those before.  The weights are read once, and held in shared memory; of a
-// sequence of more than kSelHold slots they are read again for each turn.
+// slots, and knows its place from the counts of those before.  The weights are read once, and held in
+// shared memory; of a sequence of more than kSelHold slots they are read again for each turn.
 __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEvict e, uint32_t hold) {
   extern __shared__ float held[];  // [hold]
   __shared__ uint32_t hist[kHists][kBins];
@@ -890,7 +1060,8 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(PagedKV c, PagedEvi
 
 cudaError_t launch_paged_append(const PagedKV& c, const float* k, const float* v, uint32_t rows, const uint32_t* seq,
                                 const uint32_t* pos, float* weights, cudaStream_t st) {
-  QC_BY_KIND(c.kind, (k_paged_append<T><<<rows, 256, 0, st>>>(c, k, v, seq, pos, weights)));
+  const uint32_t pieces = c.kvheads * (c.D * (c.kind == F32 ? 4 : 2) / 16), threads = pieces < 256 ? (pieces + 31) / 32 * 32 : 256;
+  QC_BY_KIND(c.kind, (k_paged_append<T><<<rows, threads, 0, st>>>(c, k, v, seq, pos, weights)));
   return cudaGetLastError();
 }
 
@@ -904,6 +1075,9 @@ cudaError_t att_prepare() {
   cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        WEIGHTS ? (int)kMaxAttSmem : Att<T, DP>::kFixed);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (WEIGHTS && e == cudaSuccess)
+    e = cudaFuncSetAttribute(k_paged_weights<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Give<T, DP>::kSmem + (int)kMaxSharedSeqs / 4);
   return e;
 }
 
@@ -937,7 +1111,12 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS>, c, r, sp);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS>, c, r, sp);
+  if (WEIGHTS && r.shared && e == cudaSuccess) {
+    k_paged_weights<T, DP><<<2 * 148, Give<T, DP>::W * 32, Give<T, DP>::kSmem + (c.n_seqs + 31) / 32 * 8, st>>>(c, r);
+    e = cudaGetLastError();
+  }
+  return e;
 }
 
 // Rows are computed at the next of these widths; the columns between are zeros in shared memory.

@@ -313,8 +313,9 @@ def test_decoding_with_a_bounded_cache(cuda_engine, torch_cuda):
         h.append(ptr(k), ptr(v), len(live), ptr(pos), seq_ptr=ptr(seq), weights_ptr=ptr(weights))
         lens[seq.long()] += 1
         row_lens = lens[seq.long()].contiguous()
-        out = torch.zeros(len(live), heads, D, device="cuda")
-        h.attention(ptr(q), heads, len(live), ptr(row_lens), ptr(out), seq_ptr=ptr(seq), weights_ptr=ptr(weights))
+        out, lse = torch.zeros(len(live), heads, D, device="cuda"), torch.zeros(len(live), heads, device="cuda")
+        h.attention(ptr(q), heads, len(live), ptr(row_lens), ptr(out), seq_ptr=ptr(seq), lse_ptr=ptr(lse),
+                    weights_ptr=ptr(weights))
         for i, s in enumerate(live):
             for kh in range(KH):
                 ref[s]["k"][kh].append(k[i, kh].half().double())
@@ -352,7 +353,7 @@ def test_captured_calls_replay_on_new_data(cuda_engine, torch_cuda):
         d = {"cache": cache, "lens": torch.tensor([200, 90, 0], dtype=torch.int32, device="cuda"),
              "k": torch.randn(3, 2, 128, device="cuda"), "v": torch.randn(3, 2, 128, device="cuda"),
              "q": torch.randn(3, 16, 128, device="cuda"), "out": torch.zeros(3, 16, 128, device="cuda"),
-             "w": torch.rand(3, 2, cache.cap, device="cuda"), "kept": torch.zeros(3, 2, 100, dtype=torch.int32, device="cuda"),
+             "lse": torch.zeros(3, 16, device="cuda"), "w": torch.rand(3, 2, cache.cap, device="cuda"), "kept": torch.zeros(3, 2, 100, dtype=torch.int32, device="cuda"),
              "new": torch.zeros(3, dtype=torch.int32, device="cuda")}
         d["after"] = d["lens"] + 1
         return d
@@ -360,10 +361,11 @@ def test_captured_calls_replay_on_new_data(cuda_engine, torch_cuda):
     def step(d, stream):
         h = d["cache"].handle(cuda_engine)
         h.append(ptr(d["k"]), ptr(d["v"]), 3, ptr(d["lens"]), weights_ptr=ptr(d["w"]), stream=stream)
-        h.attention(ptr(d["q"]), 16, 3, ptr(d["after"]), ptr(d["out"]), weights_ptr=ptr(d["w"]), stream=stream)
+        h.attention(ptr(d["q"]), 16, 3, ptr(d["after"]), ptr(d["out"]), lse_ptr=ptr(d["lse"]), weights_ptr=ptr(d["w"]),
+                    stream=stream)
         h.evict(ptr(d["w"]), ptr(d["after"]), 100, 10, ptr(d["kept"]), ptr(d["new"]), stream=stream)
 
-    names = ("out", "w", "kept", "new")
+    names = ("out", "lse", "w", "kept", "new")
     graphs = []
     for seed in (1, 2):
         d, same = make(seed), make(seed)
