@@ -169,6 +169,9 @@ int qc_sampler_sample(qc_sampler* s, const float* device_logits, uint32_t n, voi
 int qc_sampler_words(qc_sampler* s, uint32_t n, uint32_t* out);
 /* Sampler::sample on the logits of the engine's last step (no step is run). */
 int qc_engine_sample(qc_engine* e, qc_sampler* s, uint32_t* token);
+/* qc_logprobs on the logits of the engine's last step, ids and results in host memory (entropy may be NULL). */
+int qc_engine_logprobs(qc_engine* e, const uint32_t* ids, uint32_t n_ids, uint32_t top, float* logprobs, float* entropy,
+                       uint32_t* top_ids, float* top_logprobs);
 /* The chat loop with sampling (main.rs:261-282) on the device: n times, sample the current
  * logits and feed the id to the next step.  tokens_out (n ids) and logits (of the last step) may
  * be NULL.  Argument errors leave the engine as it was; a failed step resets it. */
@@ -209,6 +212,25 @@ int qc_batch_sample(qc_batch* b, qc_sampler* const* samplers, const uint32_t* se
  * tokens_out (host, may be NULL): steps x n ids, step-major. */
 int qc_batch_decode_sample(qc_batch* b, qc_sampler* const* samplers, const uint32_t* seq_ids, uint32_t n, uint32_t steps,
                            uint32_t* tokens_out);
+/* As qc_batch_create, with the sequences' caches in pages (see "paged key-value cache" below) instead of one
+ * contiguous f32 block of `context` positions each: per layer two pools of n_pages pages of `page` slots
+ * in `kind` (0 F32, 1 F16, 30 BF16), shared by all sequences.  A sequence takes pages as it grows and gives
+ * them back when it is reset; a call that needs more pages than are free fails with QC_ERR_CONTEXT and
+ * changes nothing.  weights != 0: every slot's accumulated attention weight is kept (f32, per layer, KV
+ * head and position of the context), for qc_batch_evict.  Not available on expert-parallel engines. */
+int qc_batch_create_paged(qc_engine* e, uint32_t n_seqs, uint32_t context, uint32_t kind, uint32_t page, uint32_t n_pages,
+                          int weights, qc_batch** out);
+/* Of a paged batch: the slots a sequence has cached, and the free pages (either may be NULL). */
+int qc_batch_cache(const qc_batch* b, uint32_t seq, uint32_t* cached, uint32_t* free_pages);
+/* Eviction (see qc_paged_evict) of sequence seq, or of all with 0xffffffff, in every layer: one with more
+ * than `keep` cached slots keeps the last `recent` and, of the others, those of the largest accumulated
+ * attention weight, each layer and KV head its own.  Positions go on as before (the keys keep the ones
+ * they were made with); freed pages go to the other sequences. */
+int qc_batch_evict(qc_batch* b, uint32_t seq, uint32_t keep, uint32_t recent);
+/* qc_logprobs on the latest logits of sequences seq_ids[0..n): ids ([n][n_ids], each in the vocabulary) and
+ * the results in host memory (entropy may be NULL). */
+int qc_batch_logprobs(qc_batch* b, const uint32_t* seq_ids, uint32_t n, const uint32_t* ids, uint32_t n_ids, uint32_t top,
+                      float* logprobs, float* entropy, uint32_t* top_ids, float* top_logprobs);
 /* Tokens run, device time of the steps (matvec_ms), KV and weight bytes. */
 int qc_batch_stats(const qc_batch* b, qc_stats* out);
 /* Expert parallelism of a batch (BASELINE config 5 over 2-8 GPUs: dispatch and combine of the MoE

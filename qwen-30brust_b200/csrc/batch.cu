@@ -90,18 +90,19 @@ __global__ void __launch_bounds__(512) k_b_matvec(MatDesc m, const uint8_t* __re
 }
 
 // Per token (one block): QK-norm and RoPE at its position for the query heads (in place) and the
-// key heads; the key and value rows appended to its sequence's cache (model.rs:233-243).
+// key heads; the key and value rows appended to its sequence's cache (model.rs:233-243), or, with a paged
+// cache (a.kv null), the keys left in place for launch_paged_append.
 __global__ void __launch_bounds__(256) k_b_qkprep(BatchArgs a, uint32_t layer, const float* __restrict__ q_norm,
                                                    const float* __restrict__ k_norm, float* __restrict__ q,
-                                                   const float* __restrict__ k, const float* __restrict__ v) {
+                                                   float* __restrict__ k, const float* __restrict__ v) {
   extern __shared__ __align__(16) float hv[];  // [8 warps][D]
   const uint32_t t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   const BatchTok tk = a.tok[t];
   const uint32_t D = a.D, QH = a.heads, KH = a.kvheads;
   const float2* cs = a.rope + (uint64_t)tk.pos * (D / 2);
   float* buf = hv + warp * D;
-  float* kc = seq_kv(a, tk.seq, layer, 0);
-  float* vc = seq_kv(a, tk.seq, layer, 1);
+  float* kc = a.kv ? seq_kv(a, tk.seq, layer, 0) : nullptr;
+  float* vc = a.kv ? seq_kv(a, tk.seq, layer, 1) : nullptr;
   // block (t, y): heads nw y .. nw y + nw - 1 of token t (query heads, then KV heads), one per warp
   for (uint32_t h = blockIdx.y * nw + warp; h < min(QH + KH, (blockIdx.y + 1) * nw); h += nw) {
     const bool isq = h < QH;
@@ -111,6 +112,8 @@ __global__ void __launch_bounds__(256) k_b_qkprep(BatchArgs a, uint32_t layer, c
     head_norm_rope(buf, isq ? q_norm : k_norm, D, a.eps, cs);
     if (isq)
       for (uint32_t i = lane; i < D; i += 32) q[((uint64_t)t * QH + h) * D + i] = buf[i];
+    else if (!kc)
+      for (uint32_t i = lane; i < D; i += 32) k[((uint64_t)t * KH + (h - QH)) * D + i] = buf[i];
     else {
       const uint32_t kh = h - QH;
       for (uint32_t i = lane; i < D; i += 32) {
@@ -262,7 +265,7 @@ void launch_batch_matvec(const MatDesc& m, const uint8_t* xv, uint32_t xb, uint3
 }
 
 void launch_batch_qkprep(const BatchArgs& a, uint32_t layer, const float* q_norm, const float* k_norm, float* q,
-                         const float* k, const float* v, uint32_t T, cudaStream_t s) {
+                         float* k, const float* v, uint32_t T, cudaStream_t s) {
   k_b_qkprep<<<dim3(T, (a.heads + a.kvheads + 7) / 8), 256, 8 * a.D * sizeof(float), s>>>(a, layer, q_norm, k_norm, q,
                                                                                           k, v);
 }

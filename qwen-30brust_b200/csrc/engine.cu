@@ -211,6 +211,8 @@ struct qc_engine {
   uint64_t weight_bytes = 0;
   float* d_kv = nullptr;
   uint64_t kv_bytes = 0;
+  uint8_t* d_lp = nullptr;  // log probabilities: ids and results of one call
+  uint64_t lp_bytes = 0;
   uint8_t* d_scratch = nullptr;
   qc::DevState* d_state = nullptr;
   qc::DevState h_template{};
@@ -254,6 +256,7 @@ struct qc_engine {
     if (ev1) cudaEventDestroy(ev1);
     if (h_pinned) cudaFreeHost(h_pinned);
     cudaFree(d_weights);
+    cudaFree(d_lp);
     cudaFree(d_kv);
     cudaFree(d_scratch);
     for (uint32_t q = 0; q < ep_world && q < 8; q++)
@@ -985,6 +988,51 @@ struct qc_matrix {
   }
 };
 
+namespace {
+void check_logprobs(uint32_t n, const uint32_t* ids, uint32_t n_ids, uint32_t top, const float* logprobs,
+                    const uint32_t* top_ids, const float* top_logprobs) {
+  ensure(n > 0, "empty logits");
+  ensure(top <= n && top <= qc::kMaxTop, "top must be at most 64 and at most the number of logits");
+  ensure((!n_ids || (ids && logprobs)) && (!top || (top_ids && top_logprobs)), "null argument");
+}
+
+// qc_logprobs on rows src[i] (null: row 0) of an engine's logits, ids and results on the host; *buf, of *size
+// bytes, is kept for the next call.
+void host_logprobs(qc_engine* e, const float* logits, const uint32_t* src, uint32_t rows, const uint32_t* ids, uint32_t n_ids,
+                   uint32_t top, float* lp, float* entropy, uint32_t* top_ids, float* top_lp, uint8_t** buf, uint64_t* size) {
+  const uint32_t V = e->cfg.vocab;
+  check_logprobs(V, ids, n_ids, top, lp, top_ids, top_lp);
+  for (uint64_t i = 0; i < (uint64_t)rows * n_ids; i++) ensure(ids[i] < V, "token outside vocabulary", QC_ERR_TOKEN);
+  QC_CK(cudaSetDevice(e->device));
+  const uint64_t R = rows, in = R * (1 + n_ids), need = 4 * (in + R * (n_ids + 1 + 2ull * top));
+  if (need > *size) {
+    QC_CK(cudaStreamSynchronize(e->stream));
+    cudaFree(*buf);
+    *buf = nullptr;
+    *size = 0;
+    QC_CK(cudaMalloc(buf, need));
+    *size = need;
+  }
+  uint32_t* const d_src = reinterpret_cast<uint32_t*>(*buf);
+  uint32_t* const d_ids = d_src + R;
+  float* const d_lp = reinterpret_cast<float*>(d_ids + R * n_ids);
+  float* const d_ent = d_lp + R * n_ids;
+  uint32_t* const d_top = reinterpret_cast<uint32_t*>(d_ent + R);
+  float* const d_tlp = reinterpret_cast<float*>(d_top + R * top);
+  if (src) QC_CK(cudaMemcpyAsync(d_src, src, R * 4, cudaMemcpyHostToDevice, e->stream));
+  if (n_ids) QC_CK(cudaMemcpyAsync(d_ids, ids, R * n_ids * 4, cudaMemcpyHostToDevice, e->stream));
+  const qc::LogprobArgs a{logits, src ? d_src : nullptr, rows, V, V, d_ids, n_ids, top, d_lp, d_ent, d_top, d_tlp};
+  QC_CK(qc::launch_logprobs(a, e->stream));
+  if (n_ids) QC_CK(cudaMemcpyAsync(lp, d_lp, R * n_ids * 4, cudaMemcpyDeviceToHost, e->stream));
+  if (entropy) QC_CK(cudaMemcpyAsync(entropy, d_ent, R * 4, cudaMemcpyDeviceToHost, e->stream));
+  if (top) {
+    QC_CK(cudaMemcpyAsync(top_ids, d_top, R * top * 4, cudaMemcpyDeviceToHost, e->stream));
+    QC_CK(cudaMemcpyAsync(top_lp, d_tlp, R * top * 4, cudaMemcpyDeviceToHost, e->stream));
+  }
+  QC_CK(cudaStreamSynchronize(e->stream));
+}
+}  // namespace
+
 // Several sequences decoded together (no counterpart in the reference, which runs
 // one sequence): per-sequence KV caches beside an engine's weights, and one device pass per step for
 // any mix of decode tokens and prompt chunks (batch.cu), with the MoE half on the tensor cores.
@@ -1030,6 +1078,23 @@ struct qc_batch {
   qc::MoeEp ep_set[2] = {};
   bool ep_connected = false, ep_failed = false;
   unsigned long long ep_seq = 0, ep_layers = 0;
+  // a paged cache (paged.cu) in place of d_kv: pages handed to sequences as they grow, one table for all
+  // layers.  A sequence's cached slots are its positions until an eviction; from then on they are fewer.
+  struct Pages {
+    uint32_t kind = 0, page = 0, n_pages = 0, per_seq = 0;  // per_seq: pages of a full context
+    uint64_t pool_bytes = 0;                                // of K (or V) of one layer
+    uint8_t* d_pool = nullptr;                              // [layer][K, V][pool]
+    float* d_weights = nullptr;                             // [layer][seq][kv head][slot], with eviction
+    uint32_t* d_table = nullptr;                            // [seq][per_seq]
+    uint32_t* d_rows = nullptr;                             // [3][cap]: sequence, slot, length of a pass's tokens
+    float* d_lse = nullptr;                                 // [cap][heads], with eviction
+    uint32_t *d_lens = nullptr, *d_kept = nullptr;          // [2][seq]; [seq][kv head][kept_n]
+    uint64_t kept_n = 0;
+    std::vector<uint32_t> table, cached, unused;
+  };
+  std::unique_ptr<Pages> pg;
+  uint8_t* d_lp = nullptr;  // log probabilities: rows, ids and results of one call
+  uint64_t lp_bytes = 0;
 
   ~qc_batch() {
     cudaSetDevice(e->device);
@@ -1042,6 +1107,129 @@ struct qc_batch {
     cudaFree(d_buf);
     cudaFree(d_out);
     cudaFree(d_sscr);
+    cudaFree(d_lp);
+    if (pg) {
+      cudaFree(pg->d_pool);
+      cudaFree(pg->d_weights);
+      cudaFree(pg->d_table);
+      cudaFree(pg->d_rows);
+      cudaFree(pg->d_lse);
+      cudaFree(pg->d_lens);
+      cudaFree(pg->d_kept);
+    }
+  }
+
+  // ---- paged cache ------------------------------------------------------------------------------
+  void create_pages(uint32_t kind, uint32_t page, uint32_t n_pages, bool weights) {
+    const qc_config& c = e->cfg;
+    const uint64_t seqs = n_seqs;
+    pg.reset(new Pages);
+    pg->kind = kind;
+    pg->page = page;
+    pg->n_pages = n_pages;
+    pg->per_seq = (context + page - 1) / page;
+    pg->pool_bytes = (uint64_t)n_pages * c.kvheads * page * c.head_dim * (kind == qc::F32 ? 4 : 2);
+    pg->table.assign(seqs * pg->per_seq, qc::kNoSlot);
+    pg->cached.assign(n_seqs, 0);
+    for (uint32_t i = n_pages; i-- > 0;) pg->unused.push_back(i);
+    QC_CK(cudaMalloc(&pg->d_pool, 2 * c.layers * pg->pool_bytes));
+    QC_CK(cudaMalloc(&pg->d_table, pg->table.size() * 4));
+    QC_CK(cudaMalloc(&pg->d_rows, 3ull * cap * 4));
+    QC_CK(cudaMemsetAsync(pg->d_table, 0xff, pg->table.size() * 4, e->stream));
+    if (!weights) return;
+    const uint64_t floats = seqs * c.layers * c.kvheads * pg->per_seq * page;
+    QC_CK(cudaMalloc(&pg->d_weights, floats * 4));
+    QC_CK(cudaMemsetAsync(pg->d_weights, 0, floats * 4, e->stream));
+    QC_CK(cudaMalloc(&pg->d_lse, (uint64_t)cap * c.heads * 4));
+    QC_CK(cudaMalloc(&pg->d_lens, 2ull * n_seqs * 4));
+  }
+  qc::PagedKV pages_of(uint32_t layer) const {
+    uint8_t* k = pg->d_pool + 2ull * layer * pg->pool_bytes;
+    return qc::PagedKV{pg->kind,       k,           k + pg->pool_bytes, pg->n_pages, pg->page, e->cfg.kvheads,
+                       e->cfg.head_dim, pg->d_table, n_seqs,             pg->per_seq};
+  }
+  float* weights_of(uint32_t layer) const {
+    return pg->d_weights ? pg->d_weights + (uint64_t)layer * n_seqs * e->cfg.kvheads * pg->per_seq * pg->page : nullptr;
+  }
+  // Pages that sequence q lacks for `more` further slots.
+  uint32_t pages_short(uint32_t q, uint64_t more) const {
+    const uint64_t have = (pg->cached[q] + pg->page - 1ull) / pg->page, need = (pg->cached[q] + more + pg->page - 1) / pg->page;
+    return (uint32_t)(need - have);
+  }
+  // Gives every sequence q pages for count[q] further slots (checked to be there), and the device the table.
+  void grow(const std::vector<uint32_t>& count) {
+    bool any = false;
+    for (uint32_t q = 0; q < n_seqs; q++) {
+      uint32_t at = (pg->cached[q] + pg->page - 1) / pg->page;
+      for (uint32_t n = count[q] ? pages_short(q, count[q]) : 0; n; n--, any = true) {
+        pg->table[(uint64_t)q * pg->per_seq + at++] = pg->unused.back();
+        pg->unused.pop_back();
+      }
+    }
+    if (any)
+      QC_CK(cudaMemcpyAsync(pg->d_table, pg->table.data(), pg->table.size() * 4, cudaMemcpyHostToDevice, e->stream));
+  }
+  // Sequence q keeps its first `slots` slots (and all pages of a call that failed halfway go back).
+  void shrink(uint32_t q, uint32_t slots) {
+    for (uint32_t p = (slots + pg->page - 1) / pg->page; p < pg->per_seq; p++) {
+      uint32_t& t = pg->table[(uint64_t)q * pg->per_seq + p];
+      if (t != qc::kNoSlot) pg->unused.push_back(t);
+      t = qc::kNoSlot;
+    }
+    pg->cached[q] = slots;
+  }
+  // Model::reset of one sequence (model.rs:202-208).
+  void drop(uint32_t q) {
+    pos[q] = 0;
+    if (pg) shrink(q, 0);
+  }
+  // Eviction of every sequence in `which` (0xffffffff: all) to `keep` slots, layer by layer; every layer and
+  // KV head chooses its own slots, so the sequences' slots and pages stay the same for all.
+  void evict(uint32_t which, uint32_t keep, uint32_t recent) {
+    ensure(pg && pg->d_weights, "eviction needs a paged batch with weights");
+    ensure(which < n_seqs || which == 0xffffffffu, "sequence index out of range");
+    ensure(keep > 0 && recent <= keep, "recent must be at most keep, and keep at least 1");
+    std::vector<uint32_t> lens(n_seqs, 0);
+    bool any = false;
+    for (uint32_t q = 0; q < n_seqs; q++)
+      if ((which == q || which == 0xffffffffu) && pg->cached[q] > keep) lens[q] = pg->cached[q], any = true;
+    if (!any) return;
+    QC_CK(cudaSetDevice(e->device));
+    const uint64_t kept = (uint64_t)n_seqs * e->cfg.kvheads * keep;
+    if (kept > pg->kept_n) {
+      QC_CK(cudaStreamSynchronize(e->stream));
+      cudaFree(pg->d_kept);
+      pg->d_kept = nullptr;
+      pg->kept_n = 0;
+      QC_CK(cudaMalloc(&pg->d_kept, kept * 4));
+      pg->kept_n = kept;
+    }
+    try {
+      QC_CK(cudaMemcpyAsync(pg->d_lens, lens.data(), n_seqs * 4, cudaMemcpyHostToDevice, e->stream));
+      for (uint32_t l = 0; l < e->cfg.layers; l++) {
+        float* w = weights_of(l);
+        const qc::PagedEvict ev{w, pg->d_lens, keep, recent, pg->d_table, pg->d_kept, pg->d_lens + n_seqs, w};
+        QC_CK(qc::launch_paged_evict(pages_of(l), ev, e->stream));
+      }
+      QC_CK(cudaStreamSynchronize(e->stream));
+    } catch (...) {  // some layers may have moved theirs
+      for (uint32_t q = 0; q < n_seqs; q++)
+        if (lens[q]) drop(q);
+      throw;
+    }
+    for (uint32_t q = 0; q < n_seqs; q++)
+      if (lens[q]) shrink(q, keep);
+  }
+
+  // Log probabilities of the latest logits of n sequences (host arrays, see qc_logprobs).
+  void logprobs(const uint32_t* seqs, uint32_t n, const uint32_t* ids, uint32_t n_ids, uint32_t top, float* lp, float* entropy,
+                uint32_t* top_ids, float* top_lp) {
+    ensure(n > 0 && seqs, "empty batch");
+    for (uint32_t i = 0; i < n; i++) {
+      ensure(seqs[i] < n_seqs, "sequence index out of range");
+      ensure(pos[seqs[i]] > 0, "log probabilities need the logits of a previous forward");
+    }
+    host_logprobs(e, d_last, seqs, n, ids, n_ids, top, lp, entropy, top_ids, top_lp, &d_lp, &lp_bytes);
   }
 
   // ---- expert parallelism: exchange-region handles (as qc_engine's) ---------------------------
@@ -1099,7 +1287,10 @@ struct qc_batch {
     return a;
   }
 
-  void create(qc_engine* eng, uint32_t n, uint32_t ctx) {
+  // kind: of the pages of a paged cache (page slots each, n_pages in all, weights for eviction), or kNoSlot
+  // for one contiguous f32 block a sequence.
+  void create(qc_engine* eng, uint32_t n, uint32_t ctx, uint32_t kind = qc::kNoSlot, uint32_t page = 0, uint32_t n_pages = 0,
+              bool weights = false) {
     e = eng;
     ensure(n > 0 && n <= 4096, "sequence count must be in 1..=4096");
     ensure(ctx > 0 && ctx <= e->context, "batch context must be in 1..=" + std::to_string(e->context));
@@ -1112,10 +1303,14 @@ struct qc_batch {
     ensure(D % 32 == 0 && D <= 128 && c.heads / c.kvheads <= 32, "batched attention needs head_dim <= 128 (a multiple of 32) "
            "and at most 32 query heads per KV head");
     QC_CK(cudaSetDevice(e->device));
-    kv_floats = (uint64_t)c.kvheads * ctx * D;
-    const uint64_t kv_bytes = (uint64_t)n * c.layers * 2 * kv_floats * 4;
-    QC_CK(cudaMalloc(&d_kv, kv_bytes));
-    QC_CK(cudaMemsetAsync(d_kv, 0, kv_bytes, e->stream));
+    if (kind != qc::kNoSlot) {
+      create_pages(kind, page, n_pages, weights);
+    } else {
+      kv_floats = (uint64_t)c.kvheads * ctx * D;
+      const uint64_t kv_bytes = (uint64_t)n * c.layers * 2 * kv_floats * 4;
+      QC_CK(cudaMalloc(&d_kv, kv_bytes));
+      QC_CK(cudaMemsetAsync(d_kv, 0, kv_bytes, e->stream));
+    }
     for (const qc::LayerDev& L : e->layers) {
       xb_max = std::max(xb_max, qc::xview_bytes(L.q.units, qc::uses_float_x(L.q.kind) || qc::uses_float_x(L.k.kind) ||
                                                                qc::uses_float_x(L.v.kind)));
@@ -1291,7 +1486,17 @@ struct qc_batch {
         if (!t4[2]) qc::launch_batch_matvec(L.v, d_xv, xbA, T, d_v, KD, nullptr, e->sms, s);
       }
       qc::launch_batch_qkprep(ba, l, L.q_norm, L.k_norm, d_q, d_k, d_v, T, s);
-      qc::launch_batch_attention(ba, l, d_q, d_a, T, s);
+      if (pg) {
+        const uint32_t *seq = pg->d_rows, *slot = seq + cap, *len = slot + cap;
+        QC_CK(qc::launch_paged_append(pages_of(l), d_k, d_v, T, seq, slot, weights_of(l), s));
+        const qc::PagedRows r{d_q,  c.heads,   T,
+                              seq,  len,       1.f / std::sqrt((float)c.head_dim),
+                              d_a,  pg->d_lse, weights_of(l),
+                              rows_shared};
+        QC_CK(qc::launch_paged_attention(pages_of(l), r, s));
+      } else {
+        qc::launch_batch_attention(ba, l, d_q, d_a, T, s);
+      }
       if (t4[3]) {  // x += W_o attn (model.rs:245-248)
         tc_image(d_a, nullptr, T, QD, nullptr);
         tc_project({TcOut{&e->gm(l, 3), tc_smin[4 * l + 3], d_x, d_x, H}}, T, QD);
@@ -1374,6 +1579,13 @@ struct qc_batch {
     for (uint32_t q = 0; q < n_seqs; q++)
       ensure((uint64_t)pos[q] + count[q] <= context, "context limit " + std::to_string(context) + " reached",
              QC_ERR_CONTEXT);
+    if (pg) {
+      uint64_t need = 0;
+      for (uint32_t q = 0; q < n_seqs; q++) need += count[q] ? pages_short(q, count[q]) : 0;
+      ensure(need <= pg->unused.size(), "the cache has " + std::to_string(pg->unused.size()) + " free pages, " +
+             std::to_string(need) + " are needed", QC_ERR_CONTEXT);
+    }
+    counts = count;
     tk.resize(n);
     last.assign(n, 0);
     std::vector<uint32_t> p(pos);
@@ -1384,6 +1596,24 @@ struct qc_batch {
   }
 
   bool started = false;  // a call has changed device state (its sequences are reset if it fails)
+  std::vector<uint32_t> counts;  // tokens of each sequence in the call
+  bool rows_shared = false;      // two tokens of the pass belong to one sequence
+
+  // The cache rows of a pass of T tokens (paged cache): cached[q] further slots, taken as they come.
+  void stage_rows(const qc::BatchTok* tk, uint32_t T, std::vector<uint32_t>& rows) {
+    rows.assign(3ull * cap, 0);
+    rows_shared = false;
+    std::vector<uint8_t> seen(n_seqs, 0);
+    for (uint32_t i = 0; i < T; i++) {
+      const uint32_t q = tk[i].seq, slot = pg->cached[q]++;
+      rows[i] = q;
+      rows[cap + i] = slot;
+      rows[2 * cap + i] = slot + 1;
+      rows_shared |= seen[q];
+      seen[q] = 1;
+    }
+    QC_CK(cudaMemcpyAsync(pg->d_rows, rows.data(), rows.size() * 4, cudaMemcpyHostToDevice, e->stream));
+  }
 
   // Forwards of n tokens (ids on the host); logits rows of the last token of each sequence in the
   // call to `logits` (host), in call order.
@@ -1397,6 +1627,8 @@ struct qc_batch {
     QC_CK(cudaSetDevice(e->device));
     e->grow_moe(cap);
     const uint64_t V = e->cfg.vocab;
+    std::vector<uint32_t> cache_rows;
+    if (pg) grow(counts);
     uint32_t rows_done = 0;
     cudaEvent_t t0 = e->ev0, t1 = e->ev1;
     QC_CK(cudaEventRecord(t0, e->stream));
@@ -1409,6 +1641,7 @@ struct qc_batch {
       if (toks) QC_CK(cudaMemcpyAsync(d_ids, toks + b, T * 4, cudaMemcpyHostToDevice, e->stream));
       if (!osrc.empty())
         QC_CK(cudaMemcpyAsync(d_osrc, osrc.data(), osrc.size() * 4, cudaMemcpyHostToDevice, e->stream));
+      if (pg) stage_rows(tk.data() + b, T, cache_rows);
       pass(T, (uint32_t)osrc.size());
       for (uint32_t j = 0; j < osrc.size(); j++) {
         const uint32_t sq = tk[b + osrc[j]].seq;
@@ -1481,9 +1714,21 @@ struct qc_batch {
       seen[seqs[i]] = 1;
       ensure((uint64_t)pos[seqs[i]] + steps <= context, "prompt + max-tokens exceed --ctx", QC_ERR_CONTEXT);
     }
+    if (pg) {
+      uint64_t need = 0;
+      for (uint32_t i = 0; i < n; i++) need += pages_short(seqs[i], steps);
+      ensure(need <= pg->unused.size(), "the cache has " + std::to_string(pg->unused.size()) + " free pages, " +
+             std::to_string(need) + " are needed", QC_ERR_CONTEXT);
+    }
     QC_CK(cudaSetDevice(e->device));
     stage_draws(smp, seqs, n);
     started = true;
+    std::vector<uint32_t> cache_rows;
+    if (pg) {
+      counts.assign(n_seqs, 0);
+      for (uint32_t i = 0; i < n; i++) counts[seqs[i]] = steps;
+      grow(counts);
+    }
     if (steps > out_cap) {
       cudaFree(d_out);
       d_out = nullptr;
@@ -1503,6 +1748,7 @@ struct qc_batch {
       QC_CK(cudaMemcpyAsync(d_out + (uint64_t)st * n, d_ids, n * 4, cudaMemcpyDeviceToDevice, e->stream));
       for (uint32_t i = 0; i < n; i++) tk[i] = qc::BatchTok{seqs[i], pos[seqs[i]] + st};
       QC_CK(cudaMemcpyAsync(d_tok, tk.data(), n * sizeof(qc::BatchTok), cudaMemcpyHostToDevice, e->stream));
+      if (pg) stage_rows(tk.data(), n, cache_rows);
       pass(n, n);
       for (uint32_t i = 0; i < n; i++)
         QC_CK(cudaMemcpyAsync(d_last + seqs[i] * V, d_lg + i * V, V * 4, cudaMemcpyDeviceToDevice, e->stream));
@@ -1637,7 +1883,7 @@ static int batch_call(qc_batch* b, const uint32_t* seqs, uint32_t n, F&& f) {
   const int rc = api(b->e, f);
   if (rc != QC_OK && b->started && seqs)
     for (uint32_t i = 0; i < n; i++)
-      if (seqs[i] < b->n_seqs) b->pos[seqs[i]] = 0;
+      if (seqs[i] < b->n_seqs) b->drop(seqs[i]);
   return rc;
 }
 
@@ -2004,7 +2250,7 @@ int qc_batch_reset(qc_batch* b, uint32_t seq) {
   return api(b->e, [&] {
     ensure(seq < b->n_seqs || seq == 0xffffffffu, "sequence index out of range");
     for (uint32_t q = 0; q < b->n_seqs; q++)
-      if (seq == 0xffffffffu || q == seq) b->pos[q] = 0;
+      if (seq == 0xffffffffu || q == seq) b->drop(q);
   });
 }
 
@@ -2050,12 +2296,60 @@ int qc_batch_ep_connect(qc_batch* b, const void* handles, const int* device_ids)
   });
 }
 
+int qc_batch_create_paged(qc_engine* e, uint32_t n_seqs, uint32_t context, uint32_t kind, uint32_t page, uint32_t n_pages,
+                          int weights, qc_batch** out) {
+  if (!e) return g_last_error = "null engine", QC_ERR_INVALID;
+  return api(e, [&] {
+    ensure(out, "null argument");
+    *out = nullptr;
+    ensure(e->ep_world == 1, "paged batches are not available on expert-parallel engines");
+    ensure(kind == qc::F32 || kind == qc::F16 || kind == qc::BF16, "cache pages are F32, F16 or BF16");
+    ensure(page > 0 && n_pages > 0, "empty cache");
+    ensure((uint64_t)context + page <= 0x7fffffffull, "more than 2^31 - 1 slots in a sequence");
+    ensure((uint64_t)n_pages * page <= 0xffffffffull / e->cfg.kvheads, "more than 2^32 - 1 rows in a pool");
+    std::unique_ptr<qc_batch> b(new qc_batch);
+    b->create(e, n_seqs, context, kind, page, n_pages, weights != 0);
+    *out = b.release();
+  });
+}
+
+int qc_batch_cache(const qc_batch* b, uint32_t seq, uint32_t* cached, uint32_t* free_pages) {
+  if (!b) return g_last_error = "null batch", QC_ERR_INVALID;
+  return api(b->e, [&] {
+    ensure(b->pg != nullptr, "not a paged batch");
+    ensure(seq < b->n_seqs, "sequence index out of range");
+    if (cached) *cached = b->pg->cached[seq];
+    if (free_pages) *free_pages = (uint32_t)b->pg->unused.size();
+  });
+}
+
+int qc_batch_evict(qc_batch* b, uint32_t seq, uint32_t keep, uint32_t recent) {
+  if (!b) return g_last_error = "null batch", QC_ERR_INVALID;
+  return api(b->e, [&] { b->evict(seq, keep, recent); });
+}
+
+int qc_batch_logprobs(qc_batch* b, const uint32_t* seq_ids, uint32_t n, const uint32_t* ids, uint32_t n_ids, uint32_t top,
+                      float* logprobs, float* entropy, uint32_t* top_ids, float* top_logprobs) {
+  if (!b) return g_last_error = "null batch", QC_ERR_INVALID;
+  return api(b->e, [&] { b->logprobs(seq_ids, n, ids, n_ids, top, logprobs, entropy, top_ids, top_logprobs); });
+}
+
+int qc_engine_logprobs(qc_engine* e, const uint32_t* ids, uint32_t n_ids, uint32_t top, float* logprobs, float* entropy,
+                       uint32_t* top_ids, float* top_logprobs) {
+  return api(e, [&] {
+    ensure(e, "null engine");
+    ensure(e->pos > 0, "log probabilities need the logits of a previous forward");
+    host_logprobs(e, e->sc.logits, nullptr, 1, ids, n_ids, top, logprobs, entropy, top_ids, top_logprobs, &e->d_lp, &e->lp_bytes);
+  });
+}
+
 int qc_batch_stats(const qc_batch* b, qc_stats* out) {
   if (!b) return g_last_error = "null batch", QC_ERR_INVALID;
   return api(b->e, [&] {
     ensure(out, "null argument");
     *out = b->stats;
-    out->kv_bytes = (uint64_t)b->n_seqs * b->e->cfg.layers * 2 * b->kv_floats * 4;
+    out->kv_bytes = b->pg ? 2ull * b->e->cfg.layers * b->pg->pool_bytes
+                          : (uint64_t)b->n_seqs * b->e->cfg.layers * 2 * b->kv_floats * 4;
     out->weight_bytes = b->e->weight_bytes;
     out->matvecs = ((5ull + 3ull * b->e->cfg.top) * b->e->cfg.layers + 1) * b->stats.tokens;
   });
@@ -2184,15 +2478,6 @@ int qc_paged_evict(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages
     QC_CK(qc::launch_paged_evict(c, e, static_cast<cudaStream_t>(stream)));
   });
 }
-
-namespace {
-void check_logprobs(uint32_t n, const uint32_t* ids, uint32_t n_ids, uint32_t top, const float* logprobs,
-                    const uint32_t* top_ids, const float* top_logprobs) {
-  ensure(n > 0, "empty logits");
-  ensure(top <= n && top <= qc::kMaxTop, "top must be at most 64 and at most the number of logits");
-  ensure((!n_ids || (ids && logprobs)) && (!top || (top_ids && top_logprobs)), "null argument");
-}
-}  // namespace
 
 int qc_logprobs(const float* logits, uint32_t rows, uint32_t n, uint64_t stride, const uint32_t* ids, uint32_t n_ids,
                 uint32_t top, float* logprobs, float* entropy, uint32_t* top_ids, float* top_logprobs, void* stream) {

@@ -275,7 +275,7 @@ struct BatchTok {
 };
 struct BatchArgs {
   const BatchTok* tok;  // [T] device
-  float* kv;            // [seq][layer][K, V][kvheads][ctx][head_dim]
+  float* kv;            // [seq][layer][K, V][kvheads][ctx][head_dim]; null: a paged cache
   uint64_t kv_floats;   // floats of one K (or V) block of one layer: kvheads * ctx * head_dim
   uint32_t n_layers, heads, kvheads, D, ctx;
   float eps;
@@ -294,7 +294,7 @@ void launch_batch_stage(const float* x, const uint32_t* src, uint32_t T, uint32_
 void launch_batch_matvec(const MatDesc& m, const uint8_t* xv, uint32_t xb, uint32_t T, float* y, uint64_t ystride,
                          const float* add, int sms, cudaStream_t s);
 void launch_batch_qkprep(const BatchArgs& a, uint32_t layer, const float* q_norm, const float* k_norm, float* q,
-                         const float* k, const float* v, uint32_t T, cudaStream_t s);
+                         float* k, const float* v, uint32_t T, cudaStream_t s);
 void launch_batch_attention(const BatchArgs& a, uint32_t layer, const float* q, float* out, uint32_t T, cudaStream_t s);
 void launch_batch_finite(const float* v, uint64_t n, uint32_t* flag, cudaStream_t s);
 // ---- paged key-value cache (paged.cu) ----------------------------------------------------------

@@ -6,6 +6,8 @@ This mirrors the reference crate's interface on the host side:
   Engine.decode_greedy(n)       ~ the chat loop with temperature 0 (src/main.rs:261-282)
   packed_matvec(...)            ~ Vulkan::packed_matvec (src/backend.rs:174-261)
   Matrix                        ~ a resident weight matrix for Backend::matvec
+and, without a counterpart there, several sequences at once (Batch), a paged key-value cache with eviction
+(PagedCache, Batch.paged) and log probabilities (logprobs, Engine.logprobs, Batch.logprobs).
 Errors raise QwenCudaError with the engine's message and status code.  There is
 no CPU fallback: if the library is missing, loading fails.
 """
@@ -34,6 +36,7 @@ EXPORTS = (
     "qc_batch_forward", "qc_batch_reset", "qc_batch_position", "qc_batch_logits_device", "qc_batch_sample",
     "qc_batch_decode_sample", "qc_batch_stats", "qc_batch_ep_handle", "qc_batch_ep_connect",
     "qc_paged_append", "qc_paged_attention", "qc_paged_evict", "qc_logprobs",
+    "qc_batch_create_paged", "qc_batch_cache", "qc_batch_evict", "qc_batch_logprobs", "qc_engine_logprobs",
 )
 
 
@@ -154,6 +157,11 @@ def lib() -> C.CDLL:
         L.qc_paged_append.argtypes = cache + [vp, vp, u32, vp, vp, vp, vp]
         L.qc_paged_attention.argtypes = cache + [vp, u32, u32, vp, vp, C.c_float, vp, vp, vp, vp]
         L.qc_paged_evict.argtypes = cache + [vp, vp, vp, vp, vp, u32, u32, vp, vp]
+        L.qc_batch_create_paged.argtypes = [vp, u32, u32, u32, u32, u32, i, pp]
+        L.qc_batch_cache.argtypes = [vp, u32, C.POINTER(u32), C.POINTER(u32)]
+        L.qc_batch_evict.argtypes = [vp, u32, u32, u32]
+        L.qc_batch_logprobs.argtypes = [vp, vp, u32, vp, u32, u32, vp, vp, vp, vp]
+        L.qc_engine_logprobs.argtypes = [vp, vp, u32, u32, vp, vp, vp, vp]
         L.qc_logprobs.argtypes = [vp, u32, u32, u64, vp, u32, u32, vp, vp, vp, vp, vp]
         _lib = L
     return _lib
@@ -168,6 +176,12 @@ def row_bytes(kind: int, cols: int) -> int:
     out = C.c_uint64()
     _global_check(lib().qc_row_bytes(kind, cols, C.byref(out)))
     return out.value
+
+
+def _logprob_arrays(rows: int, n_ids: int, top: int) -> tuple:
+    """Host arrays of qc_*_logprobs: log probabilities, entropy, ids and log probabilities of the likeliest."""
+    return (np.empty((rows, max(n_ids, 1)), dtype=np.float32), np.empty(rows, dtype=np.float32),
+            np.empty((rows, max(top, 1)), dtype=np.uint32), np.empty((rows, max(top, 1)), dtype=np.float32))
 
 
 def _u8(a) -> np.ndarray:
@@ -380,6 +394,15 @@ class Engine:
                                        C.byref(ms)))
         return out, ms.value
 
+    def logprobs(self, ids=(), top: int = 0):
+        """qc_engine_logprobs of the last step's logits: (log probabilities of ids, entropy, the `top` likeliest
+        ids, their log probabilities)."""
+        want = np.ascontiguousarray(ids, dtype=np.uint32).reshape(1, -1)
+        out = _logprob_arrays(1, want.shape[1], top)
+        self._check(lib().qc_engine_logprobs(self._h, want.ctypes.data, want.shape[1], top,
+                                             *[a.ctypes.data for a in out]))
+        return out[0][0, :want.shape[1]], float(out[1][0]), out[2][0, :top], out[3][0, :top]
+
     def logits_device_ptr(self) -> int:
         p = C.c_void_p()
         self._check(lib().qc_logits_device(self._h, C.byref(p)))
@@ -412,6 +435,38 @@ class Batch:
         engine._check(lib().qc_batch_create(engine._h, n_seqs, context, C.byref(h)))
         self._h, self.engine, self.n_seqs, self.context = h, engine, n_seqs, context
         self.vocab = engine.vocab
+
+    @classmethod
+    def paged(cls, engine: Engine, n_seqs: int, context: int, kind: int, page: int, n_pages: int, weights: bool = False):
+        """qc_batch_create_paged: caches in n_pages pages of `page` slots of GGML type `kind` (F32, F16 or
+        BF16: PagedCache's numbers) shared by the sequences; weights: keep what evict() goes by."""
+        h = C.c_void_p()
+        engine._check(lib().qc_batch_create_paged(engine._h, n_seqs, context, kind, page, n_pages, int(weights),
+                                                  C.byref(h)))
+        self = cls.__new__(cls)
+        self._h, self.engine, self.n_seqs, self.context = h, engine, n_seqs, context
+        self.vocab = engine.vocab
+        return self
+
+    def cache(self, seq: int) -> tuple[int, int]:
+        """Of a paged batch: (slots that sequence seq has cached, free pages)."""
+        n, f = C.c_uint32(), C.c_uint32()
+        self._check(lib().qc_batch_cache(self._h, seq, C.byref(n), C.byref(f)))
+        return n.value, f.value
+
+    def evict(self, keep: int, recent: int, seq: int = 0xFFFFFFFF) -> None:
+        """qc_batch_evict of one sequence, or of all: at most `keep` cached slots, the last `recent` among them."""
+        self._check(lib().qc_batch_evict(self._h, seq, keep, recent))
+
+    def logprobs(self, seq_ids, ids=None, top: int = 0):
+        """qc_batch_logprobs of the sequences' latest logits: (log probabilities of ids [n][n_ids], entropies [n],
+        the `top` likeliest ids [n][top], their log probabilities)."""
+        sq = np.ascontiguousarray(seq_ids, dtype=np.uint32)
+        want = np.ascontiguousarray(ids if ids is not None else np.empty((sq.size, 0)), dtype=np.uint32).reshape(sq.size, -1)
+        out = _logprob_arrays(sq.size, want.shape[1], top)
+        self._check(lib().qc_batch_logprobs(self._h, sq.ctypes.data, sq.size, want.ctypes.data, want.shape[1], top,
+                                            *[a.ctypes.data for a in out]))
+        return out[0][:, :want.shape[1]], out[1], out[2][:, :top], out[3][:, :top]
 
     def _check(self, rc: int) -> None:
         self.engine._check(rc)

@@ -169,6 +169,16 @@ pub mod ffi {
         ) -> c_int;
         pub fn qc_sampler_words(s: *mut qc_sampler, n: u32, out: *mut u32) -> c_int;
         pub fn qc_engine_sample(e: *mut qc_engine, s: *mut qc_sampler, token: *mut u32) -> c_int;
+        pub fn qc_engine_logprobs(
+            e: *mut qc_engine,
+            ids: *const u32,
+            n_ids: u32,
+            top: u32,
+            logprobs: *mut c_float,
+            entropy: *mut c_float,
+            top_ids: *mut u32,
+            top_logprobs: *mut c_float,
+        ) -> c_int;
         pub fn qc_decode_sample(
             e: *mut qc_engine,
             s: *mut qc_sampler,
@@ -204,6 +214,40 @@ pub mod ffi {
             n: u32,
             steps: u32,
             tokens_out: *mut u32,
+        ) -> c_int;
+        pub fn qc_batch_create_paged(
+            e: *mut qc_engine,
+            n_seqs: u32,
+            context: u32,
+            kind: u32,
+            page: u32,
+            n_pages: u32,
+            weights: c_int,
+            out: *mut *mut qc_batch,
+        ) -> c_int;
+        pub fn qc_batch_cache(
+            b: *const qc_batch,
+            seq: u32,
+            cached: *mut u32,
+            free_pages: *mut u32,
+        ) -> c_int;
+        pub fn qc_batch_evict(
+            b: *mut qc_batch,
+            seq: u32,
+            keep: u32,
+            recent: u32,
+        ) -> c_int;
+        pub fn qc_batch_logprobs(
+            b: *mut qc_batch,
+            seq_ids: *const u32,
+            n: u32,
+            ids: *const u32,
+            n_ids: u32,
+            top: u32,
+            logprobs: *mut c_float,
+            entropy: *mut c_float,
+            top_ids: *mut u32,
+            top_logprobs: *mut c_float,
         ) -> c_int;
         pub fn qc_batch_stats(b: *const qc_batch, out: *mut qc_stats) -> c_int;
         pub fn qc_batch_ep_handle(b: *mut qc_batch, handle: *mut c_void, device_id: *mut c_int) -> c_int;
@@ -604,6 +648,59 @@ pub mod safe {
         }
         pub fn reset(&mut self, seq: u32) -> Result<()> {
             self.engine.check(unsafe { ffi::qc_batch_reset(self.h, seq) })
+        }
+        /// As `new`, with the caches in `n_pages` pages of `page` slots of GGML type `kind` (0 F32, 1 F16,
+        /// 30 BF16) shared by the sequences; `weights`: keep what `evict` goes by.
+        pub fn paged(
+            engine: &'e mut Engine,
+            n_seqs: u32,
+            context: u32,
+            kind: u32,
+            page: u32,
+            n_pages: u32,
+            weights: bool,
+        ) -> Result<Self> {
+            let mut h = ptr::null_mut();
+            engine.check(unsafe {
+                ffi::qc_batch_create_paged(engine.h, n_seqs, context, kind, page, n_pages, weights as c_int, &mut h)
+            })?;
+            Ok(Batch { h, engine })
+        }
+        /// Of a paged batch: the slots a sequence has cached, and the free pages.
+        pub fn cache(&self, seq: u32) -> Result<(u32, u32)> {
+            let (mut cached, mut free) = (0u32, 0u32);
+            self.engine.check(unsafe { ffi::qc_batch_cache(self.h, seq, &mut cached, &mut free) })?;
+            Ok((cached, free))
+        }
+        /// At most `keep` cached slots of sequence `seq` (u32::MAX: of all), the last `recent` among them and
+        /// otherwise those of the largest accumulated attention weight.
+        pub fn evict(&mut self, seq: u32, keep: u32, recent: u32) -> Result<()> {
+            self.engine.check(unsafe { ffi::qc_batch_evict(self.h, seq, keep, recent) })
+        }
+        /// Of the latest logits of each sequence: log probabilities of `n_ids` ids each, the entropies, and
+        /// the `top` likeliest ids with theirs, sequence by sequence.
+        pub fn logprobs(&mut self, seq_ids: &[u32], ids: &[u32], top: u32) -> Result<(Vec<f32>, Vec<f32>, Vec<u32>, Vec<f32>)> {
+            let n = seq_ids.len();
+            if n == 0 || ids.len() % n != 0 {
+                return Err(Error { code: ffi::QC_ERR_INVALID, message: "ids are not a whole number a sequence".into() });
+            }
+            let (mut lp, mut ent) = (vec![0f32; ids.len()], vec![0f32; n]);
+            let (mut ti, mut tl) = (vec![0u32; n * top as usize], vec![0f32; n * top as usize]);
+            self.engine.check(unsafe {
+                ffi::qc_batch_logprobs(
+                    self.h,
+                    seq_ids.as_ptr(),
+                    n as u32,
+                    ids.as_ptr(),
+                    (ids.len() / n) as u32,
+                    top,
+                    lp.as_mut_ptr(),
+                    ent.as_mut_ptr(),
+                    ti.as_mut_ptr(),
+                    tl.as_mut_ptr(),
+                )
+            })?;
+            Ok((lp, ent, ti, tl))
         }
         /// Batches of an expert-parallel engine: this rank's exchange-region handle and GPU id.
         pub fn ep_handle(&self) -> Result<([u8; 64], i32)> {
