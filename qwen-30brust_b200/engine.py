@@ -408,7 +408,15 @@ class Engine:
         self._check(lib().qc_logits_device(self._h, C.byref(p)))
         return p.value
 
+    def _adopt(self, handle) -> None:
+        """A batch of this engine: destroyed with it if it is still there (when both are collected in one
+        garbage cycle, their finalizers run in any order)."""
+        self.__dict__.setdefault("_batches", set()).add(handle.value)
+
     def close(self) -> None:
+        """Destroys the engine, and its batches first."""
+        for b in self.__dict__.pop("_batches", ()):
+            lib().qc_batch_destroy(b)
         if getattr(self, "_h", None):
             lib().qc_engine_destroy(self._h)
             self._h = None
@@ -433,6 +441,7 @@ class Batch:
     def __init__(self, engine: Engine, n_seqs: int, context: int):
         h = C.c_void_p()
         engine._check(lib().qc_batch_create(engine._h, n_seqs, context, C.byref(h)))
+        engine._adopt(h)
         self._h, self.engine, self.n_seqs, self.context = h, engine, n_seqs, context
         self.vocab = engine.vocab
 
@@ -444,6 +453,7 @@ class Batch:
         engine._check(lib().qc_batch_create_paged(engine._h, n_seqs, context, kind, page, n_pages, int(weights),
                                                   C.byref(h)))
         self = cls.__new__(cls)
+        engine._adopt(h)
         self._h, self.engine, self.n_seqs, self.context = h, engine, n_seqs, context
         self.vocab = engine.vocab
         return self
@@ -534,7 +544,10 @@ class Batch:
 
     def close(self) -> None:
         if getattr(self, "_h", None):
-            lib().qc_batch_destroy(self._h)
+            live = self.engine.__dict__.get("_batches", set())
+            if self._h.value in live:  # (else the engine has taken it along)
+                live.remove(self._h.value)
+                lib().qc_batch_destroy(self._h)
             self._h = None
 
     def __del__(self):
