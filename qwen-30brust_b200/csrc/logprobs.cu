@@ -96,7 +96,7 @@ template <int VEC>
 constexpr uint32_t kLpSmem = sizeof(LpShared) + kLpWarps * kLpAhead * VEC * 512 > sizeof(LpShared) + kLpWarps * kLpKeep * 8
                                  ? sizeof(LpShared) + kLpWarps * kLpAhead * VEC * 512
                                  : sizeof(LpShared) + kLpWarps * kLpKeep * 8;
-static_assert(sizeof(LpShared) % 16 == 0, "chunks are 16-byte aligned");
+static_assert(kLpKeep * kLpWarps % kLpThreads == 0 && sizeof(LpShared) % 16 == 0, "chunks are 16-byte aligned");
 
 // 2^x to 2 ulp (results below 2^-126 are 0)
 __device__ __forceinline__ float pow2(float x) {
@@ -105,17 +105,63 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
-// The keys of list[0, n) by size, the k largest to sh.best (keys differ): four lanes count a key's larger ones.
-__device__ __forceinline__ void select_best(LpShared& sh, const unsigned long long* list, uint32_t n, uint32_t k) {
+// The k largest of list[0, n), sorted, to sh.best (n <= 4 kLpThreads, the keys differ).  Of many keys first
+// those whose value reaches the k-th largest's, up to ten bits behind the bits that all share; then a key's
+// place is the number of larger ones, which four lanes count.  `other` has room for n keys.
+__device__ __forceinline__ void select_best(LpShared& sh, const unsigned long long* list, unsigned long long* other, uint32_t n,
+                                            uint32_t k) {
+  const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  if (n > 96 && n > k) {
+    uint32_t key[kLpKeep * kLpWarps / kLpThreads], hi = 0, lo = 0xffffffffu;
+#pragma unroll
+    for (uint32_t u = 0; u < kLpKeep * kLpWarps / kLpThreads; u++) {
+      key[u] = tid + u * kLpThreads < n ? (uint32_t)(list[tid + u * kLpThreads] >> 32) : 0;
+      hi = max(hi, key[u]);
+      if (tid + u * kLpThreads < n) lo = min(lo, key[u]);
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    if (lane == 0) {
+      sh.shown[0][warp] = hi;
+      sh.shown[0][kLpWarps + warp] = lo;
+    }
+    if (tid == 0) sh.warp_n[0] = 0;
+    __syncthreads();
+    for (uint32_t v = 0; v < kLpWarps; v++) {
+      hi = max(hi, sh.shown[0][v]);
+      lo = min(lo, sh.shown[0][kLpWarps + v]);
+    }
+    const int same = hi == lo ? 32 : __clz(hi ^ lo), end = max(0, 32 - same - 10);
+    uint32_t T = same ? hi & ~(0xffffffffu >> (same - 1) >> 1) : 0, turn = 1;
+    for (int b = 31 - same; b >= end; b--, turn = 3 - turn) {  // (counts alternate between two places)
+      uint32_t count = 0;
+#pragma unroll
+      for (uint32_t u = 0; u < kLpKeep * kLpWarps / kLpThreads; u++)
+        count += tid + u * kLpThreads < n && key[u] >= (T | 1u << b);
+      count = __reduce_add_sync(0xffffffffu, count);
+      if (lane == 0) sh.shown[turn][warp] = count;
+      __syncthreads();
+      count = 0;
+#pragma unroll
+      for (uint32_t v = 0; v < kLpWarps; v++) count += sh.shown[turn][v];
+      if (count >= k) T |= 1u << b;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kLpKeep * kLpWarps / kLpThreads; u++)
+      if (tid + u * kLpThreads < n && key[u] >= T) other[atomicAdd(&sh.warp_n[0], 1)] = list[tid + u * kLpThreads];
+    __syncthreads();
+    n = sh.warp_n[0];
+    list = other;
+  }
   for (uint32_t i0 = 0; i0 < n; i0 += kLpThreads / 4) {
-    const uint32_t i = i0 + threadIdx.x / 4;
+    const uint32_t i = i0 + tid / 4;
     const unsigned long long x = i < n ? list[i] : 0;
     uint32_t above = 0;
 #pragma unroll 8
-    for (uint32_t j = threadIdx.x % 4; j < n; j += 4) above += list[j] > x;
+    for (uint32_t j = tid % 4; j < n; j += 4) above += list[j] > x;
     above += __shfl_xor_sync(0xffffffffu, above, 1);
     above += __shfl_xor_sync(0xffffffffu, above, 2);
-    if (i < n && above < k && threadIdx.x % 4 == 0) sh.best[above] = x;
+    if (i < n && above < k && tid % 4 == 0) sh.best[above] = x;
   }
   __syncthreads();
 }
@@ -332,10 +378,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(LogprobArgs a, uint3
       fetch(base + (kLpAhead + 1) * kStep, round + 1 + kLpAhead);
     }
   }
-  if (kept > max(k, 32u)) {
-    shrink(mine, kept, k);
-    kept = k;
-  }
   asm volatile("cp.async.wait_all;" ::: "memory");  // (nothing lands where the candidates go)
 
   // the warps' parts and candidates
@@ -361,7 +403,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(LogprobArgs a, uint3
     unsigned long long* const list = reinterpret_cast<unsigned long long*>(behind);
     for (uint32_t i = lane; i < kept; i += 32) list[at + i] = mine[i];
     __syncthreads();
-    select_best(sh, list, all, k);
+    select_best(sh, list, sh.kept[0], all, k);  // (the kept keys are all in the list)
     have = min(all, k);
   }
   // the block's, to every block
