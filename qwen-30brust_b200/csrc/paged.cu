@@ -106,10 +106,10 @@ struct Att {
   static constexpr int W = 8 * kStage <= kRoom ? 4 : 2;
   static constexpr int kFit = kRoom / (W * kStage);
   static constexpr int NS = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
-  static constexpr int kRing = W * NS * kStage;
+  static constexpr int kWide = 200 * 1024 / (NS * kStage) > 8 ? 8 : 200 * 1024 / (NS * kStage);  // one block an SM
   static constexpr int kO = DP + 4;                                // floats between two heads' O in a warp's part
-  // ring; this block's share of every block's O; every block's 8 maxima and 8 sums; the warps' maxima
-  static constexpr int kFixed = kRing + 8 * DP * 4 + kMaxCluster * 16 * 4 + W * 8 * 4;
+  // ring of w warps; this block's share of every block's O; every block's 8 maxima and 8 sums; the warps' maxima
+  static constexpr int fixed(int w) { return w * NS * kStage + 8 * DP * 4 + kMaxCluster * 16 * 4 + w * 8 * 4; }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -194,6 +194,11 @@ __device__ __forceinline__ void st_cluster(uint32_t a, float v) {
 __device__ __forceinline__ void st_cluster4(uint32_t a, float4 v) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
+}
+__device__ __forceinline__ uint2 ld_cluster2(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
 }
 // 2^x to 2 ulp (results below 2^-126 are 0)
 __device__ __forceinline__ float pow2(float x) {
@@ -381,13 +386,13 @@ struct AttSplit {
   uint32_t logc, step_pages, step_slots, score_tiles;
 };
 
-template <class T, int DP, bool WEIGHTS>
-__global__ void __launch_bounds__(Att<T, DP>::W * 32, Att<T, DP>::kFixed <= 75 * 1024 ? 3 : 1)
+template <class T, int DP, bool WEIGHTS, int W>
+__global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 : 1)
     k_paged_attention(PagedKV c, PagedRows r, AttSplit sp) {
   using A = Att<T, DP>;
-  constexpr int W = A::W, NS = A::NS;
+  constexpr int NS = A::NS;
   extern __shared__ __align__(16) uint8_t sm[];
-  float* const in_o = reinterpret_cast<float*>(sm + A::kRing);  // [C][8 DP / C]: this block's share of every block's O
+  float* const in_o = reinterpret_cast<float*>(sm + W * NS * A::kStage);  // [C][8 DP / C]: this block's share of every block's O
   float* const in_m = in_o + 8 * DP;                            // [C][16]: every block's maxima, sums
   float* const warp_m = in_m + kMaxCluster * 16;                // [W][8]
   const uint32_t C = 1u << sp.logc, rank = blockIdx.x & (C - 1), h = blockIdx.y, i = blockIdx.x >> sp.logc;
@@ -404,8 +409,9 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32, Att<T, DP>::kFixed <= 75 *
     give = !__syncthreads_or(other);
   }
   const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
-  // Where pages hold whole runs of 8 positions (RUNS) a lane copies its part of a run with one address;
-  // else every position has its own page and its lanes ask the lane that looked it up.
+  // Where pages hold whole runs of 8 positions a lane copies its part of a run with one address; else every
+  // position has its own page and its lanes ask the lane that looked it up.  64 sequences of 4096
+  // positions in bf16: 100 us with pages of 16 slots (runs), 105 with pages of 250.
   const bool runs = c.page % 8 == 0;
   const uint32_t step = C * W * kTile, gw = rank * W + warp;
   const uint32_t ahead = runs ? lane / 16 * 8 : lane % kTile;  // the position of a tile this lane looks up
@@ -496,7 +502,7 @@ __global__ void __launch_bounds__(Att<T, DP>::W * 32, Att<T, DP>::kFixed <= 75 *
     float o[DP / 16][4], m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
 #pragma unroll
     for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
-    float4* const kept_scores = reinterpret_cast<float4*>(sm + A::kFixed) + (uint64_t)warp * sp.score_tiles * 32 + lane;
+    float4* const kept_scores = reinterpret_cast<float4*>(sm + A::fixed(W)) + (uint64_t)warp * sp.score_tiles * 32 + lane;
     auto masked_scores = [&](uint32_t n, uint32_t ktile, float (&x)[4]) {
       q.scores(ktile, x);
       const uint32_t pos = gw * kTile + n * step + g;
@@ -845,7 +851,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 constexpr uint32_t kSelThreads = 1024, kSelWarps = kSelThreads / 32;
 constexpr uint32_t kSelHold = 40960;  // slots whose weights a block holds in shared memory
-constexpr uint32_t kHists = 4, kBins = 2048;
+constexpr uint32_t kHists = 4, kBins = 2048, kSelBlocks = 8;
+static_assert(kBins == 2 * kSelThreads, "two bins a thread");
 
 // The slots that (sequence, KV head) keeps, ascending, to kept[..][keep]; kNoSlot behind them, and in
 // the first place when the sequence's length or pages are invalid.  Their weights to weights_out.
@@ -853,18 +860,23 @@ constexpr uint32_t kHists = 4, kBins = 2048;
 // The want-th largest key is found by its first 11, next 11 and last 10 bits: a histogram of the keys that
 // share the bits found so far (four, for every fourth lane: the first bits bunch up), then a scan over its
 // bins.  Then the slots above it and the first ones at it are numbered: each thread counts its run of
-// slots, and knows its place from the counts of those before.  The weights are read once, and held in
-// shared memory; of a sequence of more than kSelHold slots they are read again for each turn.
-__global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEvict e, uint32_t hold) {
+// slots, and knows its place from the counts of those before.  A cluster of 2^logc blocks shares a
+// sequence's slots, the histograms and counts through distributed shared memory: one block alone issues
+// its instructions for long (a sequence of 20,011 slots, 4 KV heads, with its rows' move: 25.0 us with 1
+// block, 19.9 with 8).  The weights are read once, and held in shared memory; of a sequence that does not
+// fit they are read again for each turn.
+__global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEvict e, uint32_t hold, uint32_t logc) {
   extern __shared__ float held[];  // [hold]
-  __shared__ uint32_t hist[kHists][kBins];
+  __shared__ __align__(16) uint32_t hist[kHists][kBins];
   __shared__ uint32_t warp_n[2][kSelWarps];
-  __shared__ uint32_t s_bin, s_left;
-  const uint32_t s = blockIdx.x / c.kvheads, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  __shared__ uint32_t s_bin, s_left, s_sums[kSelBlocks][kSelWarps];
+  __shared__ __align__(8) uint2 s_total[2], s_bins[kSelBlocks][32];
+  const uint32_t C = 1u << logc, rank = blockIdx.x & (C - 1), unit = blockIdx.x >> logc;
+  const uint32_t s = unit / c.kvheads, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t n = e.len[s], cap = c.max_pages * c.page, m = min(n, e.keep);
-  uint32_t* const kept = e.kept + (uint64_t)blockIdx.x * e.keep;
-  const float* w = e.weights + (uint64_t)blockIdx.x * cap;
-  float* wo = e.weights_out + (uint64_t)blockIdx.x * cap;
+  uint32_t* const kept = e.kept + (uint64_t)unit * e.keep;
+  const float* w = e.weights + (uint64_t)unit * cap;
+  float* wo = e.weights_out + (uint64_t)unit * cap;
   bool bad = n > cap;
   if (!bad) {
     for (uint32_t p = tid; p < (n + c.page - 1) / c.page; p += kSelThreads)
@@ -872,7 +884,14 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
     for (uint32_t p = tid; p < (m + c.page - 1) / c.page; p += kSelThreads)
       bad |= e.dst_table[(uint64_t)s * c.max_pages + p] >= c.n_pages;
   }
-  const bool all = n <= e.keep, fits = n <= hold;
+  // the slots go by chunks that the cluster holds at once, a run of each to a block
+  const uint32_t chunk = hold << logc;
+  const bool all = n <= e.keep, fits = n <= chunk;
+  auto mine = [&](uint32_t first, uint32_t& from, uint32_t& count) {  // this block's run of the chunk at `first`
+    const uint32_t in = min(chunk, n - first), per = (in + C - 1) >> logc, at = min(in, rank * per);
+    from = first + at;
+    count = min(per, in - at);
+  };
   auto hold_weights = [&](uint32_t from, uint32_t count) {  // (eight reads on their way at a time)
     for (uint32_t i0 = tid; i0 < count; i0 += 8 * kSelThreads) {
       float x[8];
@@ -883,10 +902,14 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
         if (i0 + u * kSelThreads < count) held[i0 + u * kSelThreads] = x[u];
     }
   };
-  if (!all && fits && n <= cap) hold_weights(0, n);
+  uint32_t from = 0, count = 0;
+  if (!all && fits && n <= cap) {
+    mine(0, from, count);
+    hold_weights(from, count);
+  }
   bad = __syncthreads_or(bad);
-  if (bad || all) {
-    for (uint32_t i = tid; i < e.keep; i += kSelThreads) {
+  if (bad || all) {  // (the whole cluster)
+    for (uint32_t i = rank * kSelThreads + tid; i < e.keep; i += kSelThreads << logc) {
       kept[i] = !bad && i < n ? i : kNoSlot;
       if (!bad && i < n && wo != w) wo[i] = w[i];
     }
@@ -912,56 +935,91 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
     const uint32_t bits = shift ? 11 : 10;
     for (uint32_t i = tid; i < kHists * kBins; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (uint32_t i = tid; i < old; i += kSelThreads) {
-      const uint32_t k = weight_key(fits ? held[i] : w[i]);
+    auto add = [&](float x) {
+      const uint32_t k = weight_key(x);
       if (shift == 21 || (k ^ T) >> (shift + bits) == 0) atomicAdd(&hist[lane % kHists][k >> shift & ((1u << bits) - 1)], 1);
+    };
+    if (fits) {
+#pragma unroll 4
+      for (uint32_t i = tid; i < count; i += kSelThreads)
+        if (from + i < old) add(held[i]);
+    } else {
+#pragma unroll 4
+      for (uint32_t i = rank * kSelThreads + tid; i < old; i += kSelThreads << logc) add(w[i]);
     }
     __syncthreads();
-    // bins b, b - 1 (larger keys first: thread 0 has the last two)
+    // a warp has 64 bins, a lane two of them (b and b - 1), larger keys first.  The blocks exchange the warps'
+    // sums, and then the bins of the one warp that has the bin in question.
     const uint32_t b = kBins - 1 - 2 * tid;
     uint32_t c1 = 0, c0 = 0;
 #pragma unroll
     for (uint32_t v = 0; v < kHists; v++) {
-      c1 += hist[v][b];
-      c0 += hist[v][b - 1];
+      const uint2 x = *reinterpret_cast<const uint2*>(&hist[v][b - 1]);
+      c0 += x.x;
+      c1 += x.y;
     }
-    uint32_t sum = c1 + c0;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += y;
+    uint32_t total = __reduce_add_sync(0xffffffffu, c0 + c1);
+    if (C > 1) {
+      if (lane < C) st_cluster(cluster_addr(smem_addr(&s_sums[rank][warp]), lane), __uint_as_float(total));
+      cluster_sync();
+      total = 0;
+      for (uint32_t k = 0; k < C; k++) total += s_sums[k][warp];
     }
-    uint32_t before = __shfl_sync(0xffffffffu, sum, 31), none = 0, u0, u1;
+    uint32_t before = total, none = 0, u0, u1;
     scan(before, none, u0, u1);
-    const uint32_t above = before + sum - c1 - c0;  // keys in the bins before these two
-    if (above < left && above + c1 + c0 >= left) {
-      const bool second = above + c1 < left;
-      s_bin = b - second;
-      s_left = left - above - (second ? c1 : 0);
+    const bool hit = before < left && before + total >= left;  // (the same warp in all blocks)
+    if (C > 1) {
+      if (hit)
+        for (uint32_t k = 0; k < C; k++) {
+          const uint32_t to = cluster_addr(smem_addr(&s_bins[rank][lane]), k);
+          st_cluster(to, __uint_as_float(c0));
+          st_cluster(to + 4, __uint_as_float(c1));
+        }
+      cluster_sync();
+      if (hit) {
+        c0 = c1 = 0;
+        for (uint32_t k = 0; k < C; k++) {
+          c0 += s_bins[k][lane].x;
+          c1 += s_bins[k][lane].y;
+        }
+      }
+    }
+    if (hit) {
+      uint32_t sum = c1 + c0;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const uint32_t above = before + sum - c1 - c0;  // keys in the bins before these two
+      if (above < left && above + c1 + c0 >= left) {
+        const bool second = above + c1 < left;
+        s_bin = b - second;
+        s_left = left - above - (second ? c1 : 0);
+      }
     }
     __syncthreads();
     T |= s_bin << shift;
     left = s_left;
   }
-  uint32_t base = 0, ties = 0;  // kept so far; slots at T so far
-  for (uint32_t first = 0; first < n; first += hold) {
-    const uint32_t count = min(hold, n - first);
+  uint32_t base = 0, ties = 0, turn = 0;  // kept so far; slots at T so far
+  for (uint32_t first = 0; first < n; first += chunk, turn ^= 1) {
     if (!fits) {
-      hold_weights(first, count);
-      __syncthreads();  // (read before any of these are written; what is written lies below all that is read later)
+      mine(first, from, count);
+      hold_weights(from, count);
+      __syncthreads();
     }
     // a thread takes a run of slots (of an odd length: the threads then read from different banks)
     const uint32_t run = (count + kSelThreads - 1) / kSelThreads | 1, r0 = min(count, tid * run), r1 = min(count, r0 + run);
-    auto above = [&](uint32_t i, uint32_t k) { return first + i >= old || (want && k > T); };
-    auto tie = [&](uint32_t i, uint32_t k) { return first + i < old && want && k == T; };
+    auto above = [&](uint32_t i, uint32_t k) { return from + i >= old || (want && k > T); };
+    auto tie = [&](uint32_t i, uint32_t k) { return from + i < old && want && k == T; };
     uint32_t a = 0, t = 0, all_a, all_t;
     for (uint32_t i = r0; i < r1; i++) {
       const uint32_t k = weight_key(held[i]);
       a += above(i, k);
       t += tie(i, k);
     }
-    uint32_t sa = a, st = t;  // up to and with this thread, in the warp; then in the block, without it
+    uint32_t sa = a, st = t;  // up to and with this thread, in the warp
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const uint32_t ya = __shfl_up_sync(0xffffffffu, sa, o), yt = __shfl_up_sync(0xffffffffu, st, o);
@@ -972,6 +1030,22 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
     }
     uint32_t wa = __shfl_sync(0xffffffffu, sa, 31), wt = __shfl_sync(0xffffffffu, st, 31);
     scan(wa, wt, all_a, all_t);
+    // the blocks before this one.  (Past this barrier the whole chunk is read, so its slots may be written:
+    // what a chunk writes lies below all that later ones read.)
+    if (C > 1) {
+      if (tid == 0) s_total[turn] = make_uint2(all_a, all_t);
+      cluster_sync();
+      all_a = all_t = 0;
+      for (uint32_t k = 0; k < C; k++) {
+        const uint2 x = ld_cluster2(cluster_addr(smem_addr(&s_total[turn]), k));
+        if (k < rank) {
+          wa += x.x;
+          wt += x.y;
+        }
+        all_a += x.x;
+        all_t += x.y;
+      }
+    }
     const uint32_t ties_in = min(ties, left);
     uint32_t ties_at = ties + wt + st - t, to = base + wa + sa - a + min(ties_at, left) - ties_in;
     for (uint32_t i = r0; i < r1; i++) {
@@ -979,7 +1053,7 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
       const bool at_T = tie(i, k);
       // (the ties that stay come among the others in slot order: as many before this one as fit)
       if (above(i, k) || (at_T && ties_at < left)) {
-        kept[to] = first + i;
+        kept[to] = from + i;
         wo[to] = held[i];
         to++;
       }
@@ -989,6 +1063,7 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
     ties += all_t;
     __syncthreads();
   }
+  if (C > 1) cluster_sync();  // (the others have read this block's counts)
 }
 
 // Rows kept[i] of K or V to slot i, in 16-byte pieces: block (x: sequence and KV head; y:
@@ -1069,41 +1144,35 @@ namespace {
 
 constexpr uint32_t kMaxAttSmem = 220 * 1024;
 
-template <class T, int DP, bool WEIGHTS>
+template <class T, int DP, bool WEIGHTS, int W>
 cudaError_t att_prepare() {
-  auto* f = k_paged_attention<T, DP, WEIGHTS>;
+  using A = Att<T, DP>;
+  auto* f = k_paged_attention<T, DP, WEIGHTS, W>;
   cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       WEIGHTS ? (int)kMaxAttSmem : Att<T, DP>::kFixed);
+                                       WEIGHTS ? (int)kMaxAttSmem : A::fixed(W));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (WEIGHTS && e == cudaSuccess)
-    e = cudaFuncSetAttribute(k_paged_weights<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Give<T, DP>::kSmem + (int)kMaxSharedSeqs / 4);
   return e;
 }
 
-// Blocks of a cluster: enough that the launch fills the GPU (three blocks an SM) twice over, as the
-// sequences' lengths differ and are not known here, as long as a warp keeps four tiles of a full cache.
-template <class T, int DP, bool WEIGHTS>
-cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
+// A cluster of 2^logc blocks of W warps a (row, KV head).
+template <class T, int DP, bool WEIGHTS, int W>
+cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t logc, uint32_t tiles, cudaStream_t st) {
   using A = Att<T, DP>;
-  const uint32_t units = r.rows * c.kvheads, tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
-  AttSplit sp{};
-  while (sp.logc < 4 && tiles > A::W << sp.logc &&
-         ((units << sp.logc) < 148 || ((units << sp.logc) < 1024 && tiles >= (12 * A::W) << sp.logc)))
-    sp.logc++;
+  static_assert(A::fixed(W) <= (int)kMaxAttSmem, "shared memory of a block");
+  AttSplit sp{logc, 0, 0, 0};
   if (WEIGHTS) {
-    const uint32_t room = (kMaxAttSmem - A::kFixed) / (A::W * 512);
-    auto per_warp = [&] { return (tiles + (A::W << sp.logc) - 1) / (A::W << sp.logc); };
+    const uint32_t room = (kMaxAttSmem - A::fixed(W)) / (W * 512);
+    auto per_warp = [&] { return (tiles + (W << sp.logc) - 1) / (W << sp.logc); };
     while (sp.logc < 4 && per_warp() > room) sp.logc++;
     sp.score_tiles = per_warp() < room ? per_warp() : room;
   }
-  const uint32_t step = (A::W * kTile) << sp.logc;
+  const uint32_t step = (W * kTile) << sp.logc;
   sp.step_pages = step / c.page;
   sp.step_slots = step % c.page;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(r.rows << sp.logc, c.kvheads);
-  cfg.blockDim = dim3(A::W * 32);
-  cfg.dynamicSmemBytes = A::kFixed + sp.score_tiles * A::W * 512;
+  cfg.blockDim = dim3(W * 32);
+  cfg.dynamicSmemBytes = A::fixed(W) + sp.score_tiles * W * 512;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1111,7 +1180,24 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS>, c, r, sp);
+  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS, W>, c, r, sp);
+}
+
+// Blocks of a cluster, and warps of a block.  Where the largest clusters leave SMs to spare, as many as there
+// are tiles for, and wide blocks (one sequence of 32,768 positions in bf16, 4 KV heads: 41.7 us with 4 warps,
+// 28.7 with 8).  Else enough small blocks to fill the GPU (three an SM) twice over, as the sequences'
+// lengths differ and are not known here, as long as a warp keeps six tiles of a full cache.
+template <class T, int DP, bool WEIGHTS>
+cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
+  using A = Att<T, DP>;
+  const uint32_t units = r.rows * c.kvheads, tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
+  uint32_t logc = 0;
+  while (logc < 4 && tiles > (uint32_t)A::W << logc &&
+         ((units << logc) < 148 || ((units << logc) < 1024 && tiles >= (12u * A::W) << logc)))
+    logc++;
+  cudaError_t e = (units << logc) <= 148 && tiles > (uint32_t)A::W << logc
+                      ? att_launch<T, DP, WEIGHTS, A::kWide>(c, r, logc, tiles, st)
+                      : att_launch<T, DP, WEIGHTS, A::W>(c, r, logc, tiles, st);
   if (WEIGHTS && r.shared && e == cudaSuccess) {
     k_paged_weights<T, DP><<<2 * 148, Give<T, DP>::W * 32, Give<T, DP>::kSmem + (c.n_seqs + 31) / 32 * 8, st>>>(c, r);
     e = cudaGetLastError();
@@ -1141,8 +1227,15 @@ struct AttLaunch {
 struct AttPrepare {
   template <class T, int DP>
   cudaError_t operator()() const {
-    const cudaError_t e = att_prepare<T, DP, false>();
-    return e == cudaSuccess ? att_prepare<T, DP, true>() : e;
+    using A = Att<T, DP>;
+    cudaError_t e = att_prepare<T, DP, false, A::W>();
+    if (e == cudaSuccess) e = att_prepare<T, DP, false, A::kWide>();
+    if (e == cudaSuccess) e = att_prepare<T, DP, true, A::W>();
+    if (e == cudaSuccess) e = att_prepare<T, DP, true, A::kWide>();
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_paged_weights<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               Give<T, DP>::kSmem + (int)kMaxSharedSeqs / 4);
+    return e;
   }
 };
 
@@ -1170,8 +1263,24 @@ cudaError_t launch_paged_attention(const PagedKV& c, const PagedRows& r, cudaStr
 
 cudaError_t launch_paged_evict(const PagedKV& c, const PagedEvict& e, cudaStream_t st) {
   const uint32_t units = c.n_seqs * c.kvheads, pieces = c.D * (c.kind == F32 ? 4 : 2) / 16;
-  const uint32_t cap = c.max_pages * c.page, hold = cap < kSelHold ? cap : kSelHold;
-  k_evict_select<<<units, kSelThreads, hold * 4, st>>>(c, e, hold);
+  // blocks a sequence and KV head: to fill the GPU, of 4096 slots at least
+  const uint32_t cap = c.max_pages * c.page;
+  uint32_t logc = 0;
+  while (1u << logc < kSelBlocks && ((uint64_t)units << logc) < 148 && cap > 4096u << logc) logc++;
+  const uint32_t per = (cap + (1u << logc) - 1) >> logc, hold = per < kSelHold ? per : kSelHold;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(units << logc);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = hold * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1u << logc;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, k_evict_select, c, e, hold, logc);
+  if (err != cudaSuccess) return err;
   // Enough blocks to fill the GPU, where there are few sequences: by rows, or in place by parts of a row
   // (64 bytes at least).
   uint32_t shares = 1, tiles = 1;
