@@ -109,7 +109,7 @@ struct Att {
   static constexpr int kWide = 200 * 1024 / (NS * kStage) > 8 ? 8 : 200 * 1024 / (NS * kStage);  // one block an SM
   static constexpr int kO = DP + 4;                                // floats between two heads' O in a warp's part
   // ring of w warps; this block's share of every block's O; every block's 8 maxima and 8 sums; the warps' maxima
-  static constexpr int fixed(int w) { return w * NS * kStage + 8 * DP * 4 + kMaxCluster * 16 * 4 + w * 8 * 4; }
+  static constexpr int fixed(int w) { return w * NS * kStage + (2 * DP + kMaxCluster) * 16 + kMaxCluster * 16 * 4 + w * 8 * 4; }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -380,11 +380,11 @@ __device__ __forceinline__ void add_values(uint32_t vtile, const float (&p)[4], 
 // exp2(x - m) / l, with l's inverse; 0 where that is 0, whatever x.
 __device__ __forceinline__ float weight_of(float x, float m, float inv) { return inv == 0.f ? 0.f : pow2(x - m) * inv; }
 
-// How a launch splits a sequence: 2^logc blocks a cluster; a warp's next tile lies step_pages pages and
+// How a launch splits a sequence: the blocks of a cluster; a warp's next tile lies step_pages pages and
 // step_slots slots further; with weights, the tiles a warp keeps the scores of; whether the longest rows
 // come first.
 struct AttSplit {
-  uint32_t logc, step_pages, step_slots, score_tiles;
+  uint32_t blocks, step_pages, step_slots, score_tiles;
   bool longest_first;
 };
 constexpr uint32_t kMaxSorted = 128;  // rows
@@ -397,10 +397,12 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
   constexpr int NS = A::NS;
   extern __shared__ __align__(16) uint8_t sm[];
   float* const in_o = reinterpret_cast<float*>(sm + W * NS * A::kStage);  // [C][8 DP / C]: this block's share of every block's O
-  float* const in_m = in_o + 8 * DP;                            // [C][16]: every block's maxima, sums
+  float* const in_m = in_o + 8 * DP + 4 * kMaxCluster;                            // [C][16]: every block's maxima, sums
   float* const warp_m = in_m + kMaxCluster * 16;                // [W][8]
-  const uint32_t C = 1u << sp.logc, rank = blockIdx.x & (C - 1), h = blockIdx.y;
-  uint32_t i = blockIdx.x >> sp.logc;  // the row
+  const uint32_t C = sp.blocks, h = blockIdx.y;
+  uint32_t rank, i;  // (the row)
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(i));
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
   uint8_t* const ring = sm + warp * NS * A::kStage;
@@ -603,7 +605,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
     again = true;
     // what they add up to goes to the blocks of the cluster: a share of O to each, maxima and sums to all
     auto part = [&](uint32_t w) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage); };
-    const uint32_t share = (2 * DP) >> sp.logc;  // 16-byte pieces of O of one block
+    const uint32_t share = (2 * DP + C - 1) / C;  // 16-byte pieces of O of one block (the last may have fewer)
     for (uint32_t e = tid; e < 2 * DP; e += W * 32) {
       const uint32_t hh = e / (DP / 4), d = e % (DP / 4) * 4;
       float4 sum = *reinterpret_cast<const float4*>(part(0) + hh * A::kO + d);
@@ -643,7 +645,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
     const uint64_t row_head = (uint64_t)i * r.heads + h * G + g0;
     for (uint32_t e = tid; e < share; e += W * 32) {
       const uint32_t hh = (rank * share + e) / (DP / 4), d = (rank * share + e) % (DP / 4) * 4;
-      if (hh >= gn || d >= D) continue;
+      if (hh >= gn || d >= D) continue;  // (pieces behind the last belong to head 8)
       float M, L;
       total(hh, M, L);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1174,34 +1176,34 @@ cudaError_t att_prepare() {
   return e;
 }
 
-// A cluster of 2^logc blocks of W warps a (row, KV head).
+// A cluster of C blocks of W warps a (row, KV head).
 template <class T, int DP, bool WEIGHTS, int W>
-cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t logc, uint32_t tiles, cudaStream_t st) {
+cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_t tiles, cudaStream_t st) {
   using A = Att<T, DP>;
   static_assert(A::fixed(W) <= (int)kMaxAttSmem, "shared memory of a block");
-  AttSplit sp{logc, 0, 0, 0, false};
+  AttSplit sp{C, 0, 0, 0, false};
   if (WEIGHTS) {
     const uint32_t room = (kMaxAttSmem - A::fixed(W)) / (W * 512);
-    auto per_warp = [&] { return (tiles + (W << sp.logc) - 1) / (W << sp.logc); };
-    while (sp.logc < 4 && per_warp() > room) sp.logc++;
+    auto per_warp = [&] { return (tiles + W * sp.blocks - 1) / (W * sp.blocks); };
+    while (sp.blocks < (uint32_t)kMaxCluster && per_warp() > room) sp.blocks++;
     sp.score_tiles = per_warp() < room ? per_warp() : room;
   }
   // Where the blocks take two to three turns on the GPU, the short rows should be the last: 21 sequences of
   // 0..1531 positions in f32 29.5 -> 24.5 us, 64 of 130..4096 in bf16 60.5 -> 58.8, but 64 of 4096 each, where
   // it only delays the start, 100 -> 106; with more turns the end matters less than the start.
-  const uint32_t blocks = (r.rows * c.kvheads) << sp.logc;
+  const uint32_t blocks = r.rows * c.kvheads * sp.blocks;
   sp.longest_first = r.rows > 1 && r.rows <= kMaxSorted && blocks > 3 * 148 && blocks <= 8 * 148;
-  const uint32_t step = (W * kTile) << sp.logc;
+  const uint32_t step = W * kTile * sp.blocks;
   sp.step_pages = step / c.page;
   sp.step_slots = step % c.page;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(r.rows << sp.logc, c.kvheads);
+  cfg.gridDim = dim3(r.rows * sp.blocks, c.kvheads);
   cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = A::fixed(W) + sp.score_tiles * W * 512;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 1u << sp.logc;
+  at[0].val.clusterDim.x = sp.blocks;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
@@ -1210,19 +1212,22 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t logc, uint
 
 // Blocks of a cluster, and warps of a block.  Where the largest clusters leave SMs to spare, as many as there
 // are tiles for, and wide blocks (one sequence of 32,768 positions in bf16, 4 KV heads: 41.7 us with 4 warps,
-// 28.7 with 8).  Else enough small blocks to fill the GPU (three an SM) twice over, as the sequences'
-// lengths differ and are not known here, as long as a warp keeps six tiles of a full cache.
+// 26 with 8).  Else enough small blocks to fill the GPU (three an SM) nearly twice, as the sequences' lengths
+// differ and are not known here, as long as a warp keeps six tiles of a full cache; 24 rows of 7001 positions
+// take 106 us with 8 blocks (768 in all), 118 with 6, 136 with 16.  Large clusters leave parts of a GPC
+// unused; where they would not all find room at once, clusters that do are better (32 units of 9000..32768
+// positions: 73 us with 12 blocks, 80 with 16, 88 with 8).
 template <class T, int DP, bool WEIGHTS>
 cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   using A = Att<T, DP>;
   const uint32_t units = r.rows * c.kvheads, tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
-  uint32_t logc = 0;
-  while (logc < 4 && tiles > (uint32_t)A::W << logc &&
-         ((units << logc) < 148 || ((units << logc) < 1024 && tiles >= (12u * A::W) << logc)))
-    logc++;
-  cudaError_t e = (units << logc) <= 148 && tiles > (uint32_t)A::W << logc
-                      ? att_launch<T, DP, WEIGHTS, A::kWide>(c, r, logc, tiles, st)
-                      : att_launch<T, DP, WEIGHTS, A::W>(c, r, logc, tiles, st);
+  uint32_t C = 1;
+  while (C < (uint32_t)kMaxCluster && tiles > A::W * C &&
+         (units * C < 148 || (units * C < 700 && tiles >= 12 * A::W * C)))
+    C *= 2;
+  if (C == (uint32_t)kMaxCluster && units > 384 / C) C = 384 / units > 8 ? 384 / units : 8;
+  cudaError_t e = units * C <= 148 && tiles > A::W * C ? att_launch<T, DP, WEIGHTS, A::kWide>(c, r, C, tiles, st)
+                                                       : att_launch<T, DP, WEIGHTS, A::W>(c, r, C, tiles, st);
   if (WEIGHTS && r.shared && e == cudaSuccess) {
     k_paged_weights<T, DP><<<2 * 148, Give<T, DP>::W * 32, Give<T, DP>::kSmem + (c.n_seqs + 31) / 32 * 8, st>>>(c, r);
     e = cudaGetLastError();
