@@ -2436,7 +2436,7 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     ensure(seq || rows <= n_seqs, "more rows than sequences");
     ensure((uint64_t)rows * kvheads <= 0x7ffffffull, "too many rows");
     ensure(!weights || lse, "weights need lse");
-    ensure(!weights || !seq || n_seqs <= qc::kMaxSharedSeqs, "weights with seq: more than 131072 sequences");
+    ensure(!weights || !seq || n_seqs <= qc::kMaxSharedSeqs, "weights with seq: more than 8192 sequences");
     DevicePointers at;
     at.add(k_pages, "k_pages", 16);
     at.add(v_pages, "v_pages", 16);

@@ -317,7 +317,7 @@ struct PagedRows {
   float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights (needs lse)
   bool shared;       // with weights: several rows may name one sequence (n_seqs <= kMaxSharedSeqs)
 };
-constexpr uint32_t kMaxSharedSeqs = 1u << 17;
+constexpr uint32_t kMaxSharedSeqs = 8192;
 constexpr uint32_t kNoSlot = 0xffffffffu;
 struct PagedEvict {
   const float* weights;

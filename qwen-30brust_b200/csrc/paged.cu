@@ -718,8 +718,9 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
 // positions and goes through its sequence's rows in call order: scores again (K is read once more for all
 // rows together), weights exp(s - lse) from the rows' lse, summed over heads and rows in registers, one
 // addition to the slot at the end.  The rows' operands are split into planes once a block, a row a warp.
-// A launch has two blocks an SM; each finds the sequences that two rows or more name, in one pass over
-// seq, and ends at once when there are none.
+// A launch has two blocks an SM; each finds the sequences that two rows or more name and their longest
+// rows, in one pass over seq and len, and ends at once when there are none; their tiles go to the blocks
+// in turn.
 template <class T, int DP>
 struct Give {
   using A = Att<T, DP>;
@@ -727,7 +728,7 @@ struct Give {
   static constexpr int kWords = (A::kKS * A::kQP * 2 + 2 + 3) / 4 * 4;  // of a row's operand, a lane
   static constexpr int W = 8 * (kTileBytes + kWords * 128) <= 104 * 1024 ? 8 : 4;
   static constexpr int kList = W * 32;                                  // rows at a time
-  static constexpr int kSmem = W * (kTileBytes + kWords * 128) + W * 48 + kList * 4 + 64;  // and two bits a sequence
+  static constexpr int kSmem = W * (kTileBytes + kWords * 128) + W * 48 + kList * 4 + 64;  // and a length and two bits a sequence
 };
 
 template <class T, int DP>
@@ -741,16 +742,19 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32) k_paged_weights(PagedKV c
   uint32_t* const row_len = reinterpret_cast<uint32_t*>(row_lse + W * 8);          // [W]
   uint32_t* const list = row_len + W * 4;                                          // [kList]
   uint32_t* const warp_n = list + B::kList;                                        // [W], at most 16
-  uint32_t* const seen = warp_n + 16;
+  uint32_t* const longest_of = warp_n + 16;  // [n_seqs] (rows longer than the cache give no weights)
+  uint32_t* const seen = longest_of + c.n_seqs;
   const uint32_t words = (c.n_seqs + 31) / 32;
   uint32_t* const twice = seen + words;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
-  for (uint32_t k = tid; k < 2 * words; k += W * 32) seen[k] = 0;
+  for (uint32_t k = tid; k < c.n_seqs + 2 * words; k += W * 32) longest_of[k] = 0;
   __syncthreads();
   for (uint32_t k = tid; k < r.rows; k += W * 32) {
-    const uint32_t s = r.seq[k];
-    if (s < c.n_seqs && atomicOr(&seen[s / 32], 1u << s % 32) >> s % 32 & 1) atomicOr(&twice[s / 32], 1u << s % 32);
+    const uint32_t s = r.seq[k], n = r.len[k];
+    if (s >= c.n_seqs) continue;
+    if (atomicOr(&seen[s / 32], 1u << s % 32) >> s % 32 & 1) atomicOr(&twice[s / 32], 1u << s % 32);
+    if (n <= cap) atomicMax(&longest_of[s], n);
   }
   __syncthreads();
   uint8_t* const tile = sm + warp * B::kTileBytes;
@@ -760,19 +764,15 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32) k_paged_weights(PagedKV c
     for (uint32_t e = lane; e < kTile * extra; e += 32)
       *reinterpret_cast<uint4*>(tile + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
   }
+  uint32_t turn = 0;  // the block that gets the next sequence's first item
   for (uint32_t word = 0; word < words; word++)
     for (uint32_t bits = twice[word]; bits; bits &= bits - 1) {
       const uint32_t s = word * 32 + __ffs(bits) - 1;
       const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
-      uint32_t longest = 0;  // (rows longer than the cache give no weights)
-      for (uint32_t k = tid; k < r.rows; k += W * 32)
-        if (r.seq[k] == s && r.len[k] <= cap) longest = max(longest, r.len[k]);
-      longest = __reduce_max_sync(0xffffffffu, longest);
-      __syncthreads();
-      if (lane == 0) warp_n[warp] = longest;
-      __syncthreads();
-      for (uint32_t v = 0; v < W; v++) longest = max(longest, warp_n[v]);
-      const uint32_t blocks = (longest + W * kTile - 1) / (W * kTile);
+      const uint32_t longest = longest_of[s], blocks = (longest + W * kTile - 1) / (W * kTile), items = blocks * c.kvheads;
+      const uint32_t mine = (blockIdx.x + gridDim.x - turn) % gridDim.x;  // this block's first item
+      turn = (turn + items) % gridDim.x;
+      if (mine >= items) continue;
       for (uint32_t from = 0; from < r.rows; from += B::kList) {  // (the same warp takes a tile every time)
         const uint32_t k = from + tid;
         const bool is = k < r.rows && r.seq[k] == s;
@@ -787,7 +787,7 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32) k_paged_weights(PagedKV c
         }
         if (is) list[at + __popc(who & ((1u << lane) - 1))] = k;
         __syncthreads();
-        for (uint32_t item = n ? blockIdx.x : 0xffffffffu; item < blocks * c.kvheads; item += gridDim.x) {
+        for (uint32_t item = n ? mine : items; item < items; item += gridDim.x) {
           const uint32_t h = item / blocks, j0 = (item % blocks * W + warp) * kTile;
           const uint32_t j = j0 + lane % kTile, p = j < longest ? pages[j / c.page] : kNoSlot;
           const uint32_t row = p < c.n_pages ? (p * c.kvheads + h) * c.page + j % c.page : kNoSlot;
@@ -1226,10 +1226,13 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
          (units * C < 148 || (units * C < 700 && tiles >= 12 * A::W * C)))
     C *= 2;
   if (C == (uint32_t)kMaxCluster && units > 384 / C) C = 384 / units > 8 ? 384 / units : 8;
-  cudaError_t e = units * C <= 148 && tiles > A::W * C ? att_launch<T, DP, WEIGHTS, A::kWide>(c, r, C, tiles, st)
+  // (blocks of two warps that keep many scores would be alone on their SM, so they had better be wide: 51
+  // sequences of 715..1276 positions, 24 heads of 192 in f32, 287 -> 182 us; with few tiles they are not)
+  const bool wide = (units * C <= 148 && tiles > A::W * C) || (WEIGHTS && A::W == 2 && tiles > 4 * A::W * C);
+  cudaError_t e = wide ? att_launch<T, DP, WEIGHTS, A::kWide>(c, r, C, tiles, st)
                                                        : att_launch<T, DP, WEIGHTS, A::W>(c, r, C, tiles, st);
   if (WEIGHTS && r.shared && e == cudaSuccess) {
-    k_paged_weights<T, DP><<<2 * 148, Give<T, DP>::W * 32, Give<T, DP>::kSmem + (c.n_seqs + 31) / 32 * 8, st>>>(c, r);
+    k_paged_weights<T, DP><<<2 * 148, Give<T, DP>::W * 32, Give<T, DP>::kSmem + c.n_seqs * 4 + (c.n_seqs + 31) / 32 * 8, st>>>(c, r);
     e = cudaGetLastError();
   }
   return e;
@@ -1264,7 +1267,7 @@ struct AttPrepare {
     if (e == cudaSuccess) e = att_prepare<T, DP, true, A::kWide>();
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(k_paged_weights<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               Give<T, DP>::kSmem + (int)kMaxSharedSeqs / 4);
+                               Give<T, DP>::kSmem + (int)kMaxSharedSeqs * 4 + (int)kMaxSharedSeqs / 4);
     return e;
   }
 };

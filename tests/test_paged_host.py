@@ -58,7 +58,7 @@ def test_bad_calls_are_refused(E):
     refused(E, "null argument", c.attention, P, 4, 1, P, None)
     refused(E, "more rows than sequences", c.attention, P, 4, 4, P, P)
     refused(E, "weights need lse", c.attention, P, 4, 1, P, P, weights_ptr=P)
-    refused(E, "131072 sequences", cache(E, n_seqs=131073).attention, P, 4, 2, P, P, seq_ptr=P, lse_ptr=P, weights_ptr=P)
+    refused(E, "8192 sequences", cache(E, n_seqs=8193).attention, P, 4, 2, P, P, seq_ptr=P, lse_ptr=P, weights_ptr=P)
     refused(E, "too many rows", c.attention, P, 4, 0xffffffff, P, P, seq_ptr=P)
     refused(E, "keep must be", c.evict, P, P, 0, 0, P, P)
     refused(E, "keep must be", c.evict, P, P, 65, 0, P, P)
