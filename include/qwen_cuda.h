@@ -278,7 +278,7 @@ int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_page
  * A row of length 0 gives out 0 and lse -inf; so does one whose scores all overflow to -inf.  Slots a row
  * does not attend to may hold anything; a non-finite value among those it reads makes its results
  * non-finite.
- * weights (may be NULL; needs lse, and with seq at most 8192 sequences): [n_seqs][kvheads][max_pages *
+ * weights (may be NULL; needs lse, and n_seqs at most 8192): [n_seqs][kvheads][max_pages *
  * page] f32; the softmax weights that the rows give slot j, summed over a KV head's query heads, are added
  * to weights[s][kv head][j]; a head whose lse is NaN gives none.  The results do not depend on timing: the
  * same call gives the same bits. */

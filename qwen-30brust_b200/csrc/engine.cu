@@ -1489,10 +1489,7 @@ struct qc_batch {
       if (pg) {
         const uint32_t *seq = pg->d_rows, *slot = seq + cap, *len = slot + cap;
         QC_CK(qc::launch_paged_append(pages_of(l), d_k, d_v, T, seq, slot, weights_of(l), s));
-        const qc::PagedRows r{d_q,  c.heads,   T,
-                              seq,  len,       1.f / std::sqrt((float)c.head_dim),
-                              d_a,  pg->d_lse, weights_of(l),
-                              rows_shared};
+        const qc::PagedRows r{d_q, c.heads, T, seq, len, 1.f / std::sqrt((float)c.head_dim), d_a, pg->d_lse, weights_of(l)};
         QC_CK(qc::launch_paged_attention(pages_of(l), r, s));
       } else {
         qc::launch_batch_attention(ba, l, d_q, d_a, T, s);
@@ -1597,20 +1594,15 @@ struct qc_batch {
 
   bool started = false;  // a call has changed device state (its sequences are reset if it fails)
   std::vector<uint32_t> counts;  // tokens of each sequence in the call
-  bool rows_shared = false;      // two tokens of the pass belong to one sequence
 
   // The cache rows of a pass of T tokens (paged cache): cached[q] further slots, taken as they come.
   void stage_rows(const qc::BatchTok* tk, uint32_t T, std::vector<uint32_t>& rows) {
     rows.assign(3ull * cap, 0);
-    rows_shared = false;
-    std::vector<uint8_t> seen(n_seqs, 0);
     for (uint32_t i = 0; i < T; i++) {
       const uint32_t q = tk[i].seq, slot = pg->cached[q]++;
       rows[i] = q;
       rows[cap + i] = slot;
       rows[2 * cap + i] = slot + 1;
-      rows_shared |= seen[q];
-      seen[q] = 1;
     }
     QC_CK(cudaMemcpyAsync(pg->d_rows, rows.data(), rows.size() * 4, cudaMemcpyHostToDevice, e->stream));
   }
@@ -2436,7 +2428,7 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     ensure(seq || rows <= n_seqs, "more rows than sequences");
     ensure((uint64_t)rows * kvheads <= 0x7ffffffull, "too many rows");
     ensure(!weights || lse, "weights need lse");
-    ensure(!weights || !seq || n_seqs <= qc::kMaxSharedSeqs, "weights with seq: more than 8192 sequences");
+    ensure(!weights || n_seqs <= qc::kMaxWeightSeqs, "weights: more than 8192 sequences");
     DevicePointers at;
     at.add(k_pages, "k_pages", 16);
     at.add(v_pages, "v_pages", 16);
@@ -2448,8 +2440,7 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     at.add(lse, "lse");
     at.add(weights, "weights");
     at.enter();
-    qc::PagedRows r{q,   heads, rows,    seq,          len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale,
-                    out, lse,   weights, seq && rows > 1};
+    qc::PagedRows r{q, heads, rows, seq, len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale, out, lse, weights};
     QC_CK(qc::launch_paged_attention(c, r, static_cast<cudaStream_t>(stream)));
   });
 }

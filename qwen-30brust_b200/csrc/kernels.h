@@ -315,9 +315,8 @@ struct PagedRows {
   float scale;
   float *out, *lse;  // [rows][heads][D], [rows][heads] or null
   float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights (needs lse)
-  bool shared;       // with weights: several rows may name one sequence (n_seqs <= kMaxSharedSeqs)
 };
-constexpr uint32_t kMaxSharedSeqs = 8192;
+constexpr uint32_t kMaxWeightSeqs = 8192;  // sequences of a call with weights
 constexpr uint32_t kNoSlot = 0xffffffffu;
 struct PagedEvict {
   const float* weights;

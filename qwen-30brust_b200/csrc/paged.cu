@@ -89,8 +89,6 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __
 //
 // The warps' (maximum, sum, O) are joined in shared memory, the blocks' through the cluster's
 // distributed shared memory in a fixed order: no workspace, no atomics, the same bits every time.
-// With weights the scores stay in shared memory (512 bytes a tile) until the final maximum and sum are
-// known; tiles beyond that room are scored again.
 
 constexpr int kTile = 16;
 constexpr int kMaxCluster = 16;
@@ -377,20 +375,16 @@ __device__ __forceinline__ void add_values(uint32_t vtile, const float (&p)[4], 
   }
 }
 
-// exp2(x - m) / l, with l's inverse; 0 where that is 0, whatever x.
-__device__ __forceinline__ float weight_of(float x, float m, float inv) { return inv == 0.f ? 0.f : pow2(x - m) * inv; }
-
 // How a launch splits a sequence: the blocks of a cluster; a warp's next tile lies step_pages pages and
-// step_slots slots further; with weights, the tiles a warp keeps the scores of; whether the longest rows
-// come first.
+// step_slots slots further; whether the longest rows come first.
 struct AttSplit {
-  uint32_t blocks, step_pages, step_slots, score_tiles;
+  uint32_t blocks, step_pages, step_slots;
   bool longest_first;
 };
 constexpr uint32_t kMaxSorted = 128;  // rows
 static_assert(kMaxSorted < kMaxCluster * 16, "lengths are sorted where the maxima and sums come later");
 
-template <class T, int DP, bool WEIGHTS, int W>
+template <class T, int DP, int W>
 __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 : 1)
     k_paged_attention(PagedKV c, PagedRows r, AttSplit sp) {
   using A = Att<T, DP>;
@@ -424,12 +418,6 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
   }
   const uint32_t s = r.seq ? r.seq[i] : i, len = r.len[i];
   if (s >= c.n_seqs) return;  // (the whole cluster)
-  bool give = WEIGHTS;  // (rows that share a sequence leave their weights to k_paged_weights)
-  if (WEIGHTS && r.shared) {
-    bool other = false;
-    for (uint32_t k = tid; k < r.rows; k += W * 32) other |= k != i && r.seq[k] == s;
-    give = !__syncthreads_or(other);
-  }
   const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
   // Where pages hold whole runs of 8 positions a lane copies its part of a run with one address; else every
   // position has its own page and its lanes ask the lane that looked it up.  64 sequences of 4096
@@ -463,7 +451,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
       return (p * c.kvheads + h) * c.page + in;
     };
     // Copies the tile of positions j0.. into a ring slot; row: this lane's lookup.
-    auto fetch = [&](uint32_t slot, uint32_t row, uint32_t j0, bool with_v) {
+    auto fetch = [&](uint32_t slot, uint32_t row, uint32_t j0) {
       constexpr uint32_t kCh = DP * sizeof(T) / 16;
       const uint32_t dst = ring_a + slot * A::kStage;
       const uint8_t *kp = static_cast<const uint8_t*>(c.k), *vp = static_cast<const uint8_t*>(c.v);
@@ -480,7 +468,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
           const bool real = p < (second ? n1 : n0);
           if (DP * sizeof(T) != chunks * 16 && ch >= chunks) continue;
           copy16(dst + p * A::kRow + ch * 16, kp + o, real);
-          if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, real);
+          copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, real);
         }
       } else {
 #pragma unroll 4
@@ -490,7 +478,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
           const uint64_t o = from == kNoSlot ? 0 : (uint64_t)from * D * sizeof(T) + ch * 16;
           if (ch >= chunks) continue;
           copy16(dst + p * A::kRow + ch * 16, kp + o, from != kNoSlot);
-          if (with_v) copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, from != kNoSlot);
+          copy16(dst + (kTile + p) * A::kRow + ch * 16, vp + o, from != kNoSlot);
         }
       }
     };
@@ -516,7 +504,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
     if (chunks * 16 < DP * sizeof(T)) clear_columns(2 * NS * kTile);
 #pragma unroll
     for (int n = 0; n < NS; n++) {
-      fetch(n, row_of(pg[n], slots[n], j0), j0, true);
+      fetch(n, row_of(pg[n], slots[n], j0), j0);
       copy_commit();
       j0 += step;
     }
@@ -524,20 +512,15 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
     float o[DP / 16][4], m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
 #pragma unroll
     for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
-    float4* const kept_scores = reinterpret_cast<float4*>(sm + A::fixed(W)) + (uint64_t)warp * sp.score_tiles * 32 + lane;
-    auto masked_scores = [&](uint32_t n, uint32_t ktile, float (&x)[4]) {
-      q.scores(ktile, x);
-      const uint32_t pos = gw * kTile + n * step + g;
-      if (pos >= len) x[0] = x[1] = -INFINITY;
-      if (pos + 8 >= len) x[2] = x[3] = -INFINITY;
-    };
     for (uint32_t n = 0, slot = 0; n < mine_n; n++, slot = slot + 1 == NS ? 0 : slot + 1) {
       copy_wait<NS - 1>();
       __syncwarp();
       const uint32_t tile_a = ring_a + slot * A::kStage;
       float x[4];
-      masked_scores(n, tile_a, x);
-      if (WEIGHTS && give && n < sp.score_tiles) kept_scores[n * 32] = make_float4(x[0], x[1], x[2], x[3]);
+      q.scores(tile_a, x);
+      const uint32_t pos = gw * kTile + n * step + g;
+      if (pos >= len) x[0] = x[1] = -INFINITY;
+      if (pos + 8 >= len) x[2] = x[3] = -INFINITY;
       const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
       if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
         float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
@@ -564,7 +547,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
       l1 += p[1] + p[3];
       add_values<T, DP>(tile_a + kTile * A::kRow, p, o);
       __syncwarp();
-      fetch(slot, row_of(next, next_in, j0), j0, true);
+      fetch(slot, row_of(next, next_in, j0), j0);
       copy_commit();
       j0 += step;
       advance();
@@ -663,205 +646,144 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
           make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
       if (d == 0 && r.lse) r.lse[row_head + hh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
-    if (WEIGHTS && give) {
-      float M[2], inv[2];  // (a head whose sum is NaN, as where a page is bad, gives no weights)
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        float L;
-        total(2 * t + u, M[u], L);
-        inv[u] = 2 * t + u >= gn || !(L > 0.f) ? 0.f : 1.f / L;
-      }
-      if (mine_n > sp.score_tiles && chunks * 16 < DP * sizeof(T)) {
-        __syncwarp();
-        clear_columns(kTile);
-      }
-      float* const w = r.weights + ((uint64_t)s * c.kvheads + h) * cap;
-      // (the weights' reads first, four tiles at a time: one after the other each would wait for the last)
-      for (uint32_t n0 = 0; n0 < mine_n; n0 += 4) {
-        float old[4];
-#pragma unroll
-        for (uint32_t u = 0; u < 4; u++) {
-          const uint32_t pos = gw * kTile + (n0 + u) * step + g + 8 * t;
-          old[u] = t < 2 && n0 + u < mine_n && pos < len ? w[pos] : 0.f;
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < 4; u++) {
-          const uint32_t n = n0 + u, base = gw * kTile + n * step, pos = base + ahead;
-          if (n >= mine_n) break;
-          float x[4];
-          if (n < sp.score_tiles) {
-            const float4 y = kept_scores[n * 32];
-            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-          } else {
-            __syncwarp();
-            fetch(0, row_of(page_at(pos, pos / c.page), pos % c.page, base), base, false);
-            copy_commit();
-            copy_wait<0>();
-            __syncwarp();
-            masked_scores(n, ring_a, x);
-          }
-          float w0 = weight_of(x[0], M[0], inv[0]) + weight_of(x[1], M[1], inv[1]);
-          float w8 = weight_of(x[2], M[0], inv[0]) + weight_of(x[3], M[1], inv[1]);
-          w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
-          w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
-          w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
-          w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
-          if (t < 2 && base + g + 8 * t < len) w[base + g + 8 * t] = old[u] + (t ? w8 : w0);
-        }
-      }
-    }
   }
 }
 
-// Weights of rows that share a sequence (a prompt's tokens): the attention above leaves them out, as its
-// clusters would have to add to the same slots one after the other.  Here a warp takes a tile of 16
-// positions and goes through its sequence's rows in call order: scores again (K is read once more for all
-// rows together), weights exp(s - lse) from the rows' lse, summed over heads and rows in registers, one
-// addition to the slot at the end.  The rows' operands are split into planes once a block, a row a warp.
-// A launch has two blocks an SM; each finds the sequences that two rows or more name and their longest
-// rows, in one pass over seq and len, and ends at once when there are none; their tiles go to the blocks
-// in turn.
+// ---- accumulated weights -------------------------------------------------------------------------
+// The rows' softmax weights exp(s - lse), summed over a KV head's heads and a sequence's rows, added to the
+// slots: a second pass over K with the lse that the attention has left, so that every slot is added to
+// once, whatever rows share a sequence, and the attention need not hold its scores.  A warp takes kTiles
+// tiles of 16 positions of a (sequence, KV head) at a time and goes through the sequence's rows in call
+// order, scores again, and sums in registers; warps do not wait for one another.  Each block finds the
+// sequences that rows name and their longest rows in one pass over seq and len; their spans go to the warps
+// in turn.  (Keeping the attention's scores in shared memory instead left one block an SM for long
+// sequences: 8 of 29,292..35,385 positions, 6 heads of 64 bf16, 113 us against 58 this way; 32 of
+// 200..2500, 32 heads of 128 f16, 39 against 41.)
 template <class T, int DP>
 struct Give {
   using A = Att<T, DP>;
+  static constexpr int W = 4;
   static constexpr int kTileBytes = kTile * A::kRow;
-  static constexpr int kWords = (A::kKS * A::kQP * 2 + 2 + 3) / 4 * 4;  // of a row's operand, a lane
-  static constexpr int W = 8 * (kTileBytes + kWords * 128) <= 104 * 1024 ? 8 : 4;
-  static constexpr int kList = W * 32;                                  // rows at a time
-  static constexpr int kSmem = W * (kTileBytes + kWords * 128) + W * 48 + kList * 4 + 64;  // and a length and two bits a sequence
+  static constexpr int kFit = 17600 / kTileBytes;  // (three blocks an SM)
+  static constexpr int kTiles = kFit > 4 ? 4 : kFit < 1 ? 1 : kFit;
+  static constexpr int kSmem = W * kTiles * kTileBytes;  // and a length a sequence
 };
 
 template <class T, int DP>
-__global__ void __launch_bounds__(Give<T, DP>::W * 32) k_paged_weights(PagedKV c, PagedRows r) {
+__global__ void __launch_bounds__(Give<T, DP>::W * 32, 3) k_paged_weights(PagedKV c, PagedRows r) {
   using A = Att<T, DP>;
   using B = Give<T, DP>;
-  constexpr int W = B::W;
+  constexpr uint32_t W = B::W, kTiles = B::kTiles, kSpan = kTiles * kTile;
   extern __shared__ __align__(16) uint8_t sm[];
-  uint4* const operands = reinterpret_cast<uint4*>(sm + W * B::kTileBytes);        // [W rows][kWords / 4][32 lanes]
-  float* const row_lse = reinterpret_cast<float*>(operands + W * B::kWords * 8);   // [W][8], times log2 e; inf: no weights
-  uint32_t* const row_len = reinterpret_cast<uint32_t*>(row_lse + W * 8);          // [W]
-  uint32_t* const list = row_len + W * 4;                                          // [kList]
-  uint32_t* const warp_n = list + B::kList;                                        // [W], at most 16
-  uint32_t* const longest_of = warp_n + 16;  // [n_seqs] (rows longer than the cache give no weights)
-  uint32_t* const seen = longest_of + c.n_seqs;
-  const uint32_t words = (c.n_seqs + 31) / 32;
-  uint32_t* const twice = seen + words;
+  uint32_t* const longest_of = reinterpret_cast<uint32_t*>(sm + B::kSmem);  // [n_seqs] (rows longer than the cache give none)
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
-  for (uint32_t k = tid; k < c.n_seqs + 2 * words; k += W * 32) longest_of[k] = 0;
+  auto seq_of = [&](uint32_t k) { return r.seq ? r.seq[k] : k; };
+  for (uint32_t k = tid; k < c.n_seqs; k += W * 32) longest_of[k] = 0;
   __syncthreads();
   for (uint32_t k = tid; k < r.rows; k += W * 32) {
-    const uint32_t s = r.seq[k], n = r.len[k];
-    if (s >= c.n_seqs) continue;
-    if (atomicOr(&seen[s / 32], 1u << s % 32) >> s % 32 & 1) atomicOr(&twice[s / 32], 1u << s % 32);
-    if (n <= cap) atomicMax(&longest_of[s], n);
+    const uint32_t s = seq_of(k), n = r.len[k];
+    if (s < c.n_seqs && n <= cap) atomicMax(&longest_of[s], n);
   }
   __syncthreads();
-  uint8_t* const tile = sm + warp * B::kTileBytes;
+  uint8_t* const tile = sm + warp * kTiles * B::kTileBytes;
   const uint32_t tile_a = smem_addr(tile);
   if (chunks * 16 < DP * sizeof(T)) {
     const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
-    for (uint32_t e = lane; e < kTile * extra; e += 32)
+    for (uint32_t e = lane; e < kTiles * kTile * extra; e += 32)
       *reinterpret_cast<uint4*>(tile + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
   }
-  uint32_t turn = 0;  // the block that gets the next sequence's first item
-  for (uint32_t word = 0; word < words; word++)
-    for (uint32_t bits = twice[word]; bits; bits &= bits - 1) {
-      const uint32_t s = word * 32 + __ffs(bits) - 1;
+  // Items of a sequence: (KV head, span of positions).  All sequences' items go to the warps in turn; a lane
+  // looks at one of 32 sequences.
+  const uint32_t warps = gridDim.x * W, me = warp * gridDim.x + blockIdx.x;
+  uint32_t total = 0;  // items of the sequences before, modulo the warps
+  for (uint32_t s0 = 0; s0 < c.n_seqs; s0 += 32) {
+    const uint32_t n_lane = s0 + lane < c.n_seqs ? longest_of[s0 + lane] : 0;
+    const uint32_t items_lane = (n_lane + kSpan - 1) / kSpan * c.kvheads;
+    uint32_t upto = items_lane % warps;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const uint32_t at_lane = (total + upto - items_lane % warps) % warps;  // the warp with the sequence's first item
+    const uint32_t mine_lane = me >= at_lane ? me - at_lane : me + warps - at_lane;
+    total = (total + __shfl_sync(0xffffffffu, upto, 31)) % warps;
+    for (uint32_t bits = __ballot_sync(0xffffffffu, mine_lane < items_lane); bits; bits &= bits - 1) {
+      const int from = __ffs(bits) - 1;
+      const uint32_t s = s0 + from, longest = __shfl_sync(0xffffffffu, n_lane, from);
+      const uint32_t spans = (longest + kSpan - 1) / kSpan, items = spans * c.kvheads;
       const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
-      const uint32_t longest = longest_of[s], blocks = (longest + W * kTile - 1) / (W * kTile), items = blocks * c.kvheads;
-      const uint32_t mine = (blockIdx.x + gridDim.x - turn) % gridDim.x;  // this block's first item
-      turn = (turn + items) % gridDim.x;
-      if (mine >= items) continue;
-      for (uint32_t from = 0; from < r.rows; from += B::kList) {  // (the same warp takes a tile every time)
-        const uint32_t k = from + tid;
-        const bool is = k < r.rows && r.seq[k] == s;
-        const uint32_t who = __ballot_sync(0xffffffffu, is);
-        __syncthreads();
-        if (lane == 0) warp_n[warp] = __popc(who);
-        __syncthreads();
-        uint32_t at = 0, n = 0;
-        for (uint32_t v = 0; v < W; v++) {
-          if (v == warp) at = n;
-          n += warp_n[v];
+      for (uint32_t item = __shfl_sync(0xffffffffu, mine_lane, from); item < items; item += warps) {
+        const uint32_t h = item / spans, j0 = item % spans * kSpan;
+        float* const w = r.weights + ((uint64_t)s * c.kvheads + h) * cap;
+        float old[kTiles], w0[kTiles], w8[kTiles];  // sums of positions g and g + 8 of a tile, this lane's heads
+        uint32_t row[kTiles];
+#pragma unroll
+        for (uint32_t u = 0; u < kTiles; u++) {
+          const uint32_t j = j0 + u * kTile + lane % kTile, p = j < longest ? pages[j / c.page] : kNoSlot;
+          row[u] = p < c.n_pages ? (p * c.kvheads + h) * c.page + j % c.page : kNoSlot;
         }
-        if (is) list[at + __popc(who & ((1u << lane) - 1))] = k;
-        __syncthreads();
-        for (uint32_t item = n ? mine : items; item < items; item += gridDim.x) {
-          const uint32_t h = item / blocks, j0 = (item % blocks * W + warp) * kTile;
-          const uint32_t j = j0 + lane % kTile, p = j < longest ? pages[j / c.page] : kNoSlot;
-          const uint32_t row = p < c.n_pages ? (p * c.kvheads + h) * c.page + j % c.page : kNoSlot;
+#pragma unroll
+        for (uint32_t u = 0; u < kTiles; u++) {
           constexpr uint32_t kCh = DP * sizeof(T) / 16;
+#pragma unroll 4
           for (uint32_t e = lane; e < kTile * kCh; e += 32) {
-            const uint32_t pos = e / kCh, ch = e % kCh, src = __shfl_sync(0xffffffffu, row, pos);
+            const uint32_t pos = e / kCh, ch = e % kCh, src = __shfl_sync(0xffffffffu, row[u], pos);
             if (ch < chunks)
-              copy16(tile_a + pos * A::kRow + ch * 16,
+              copy16(tile_a + u * B::kTileBytes + pos * A::kRow + ch * 16,
                      static_cast<const uint8_t*>(c.k) + (src == kNoSlot ? 0 : (uint64_t)src * D * sizeof(T) + ch * 16),
                      src != kNoSlot);
           }
-          copy_commit();
-          float w0 = 0.f, w8 = 0.f;  // of positions j0 + g and j0 + g + 8, this lane's heads
-          for (uint32_t g0 = 0; g0 < G; g0 += 8)
-            for (uint32_t k0 = 0; k0 < n; k0 += W) {
-              __syncthreads();  // the operands before are done with
+          const uint32_t slot = j0 + u * kTile + g + 8 * t;
+          old[u] = t < 2 && slot < longest ? w[slot] : 0.f;
+          w0[u] = w8[u] = 0.f;
+        }
+        copy_commit();
+        for (uint32_t k0 = 0; k0 < r.rows; k0 += 32)
+          for (uint32_t rows = __ballot_sync(0xffffffffu, k0 + lane < r.rows && seq_of(k0 + lane) == s); rows;
+               rows &= rows - 1) {
+            const uint32_t i = k0 + __ffs(rows) - 1, len = r.len[i];
+            if (j0 >= len || len > cap) continue;
+            for (uint32_t g0 = 0; g0 < G; g0 += 8) {
+              const uint32_t gn = min(8u, G - g0);
+              const uint64_t head = (uint64_t)i * r.heads + h * G + g0;
               Query<T, DP> q;
-              if (k0 + warp < n) {
-                const uint32_t i = list[k0 + warp], gn = min(8u, G - g0);
-                const uint64_t head = (uint64_t)i * r.heads + h * G + g0;
-                q.fetch(r.q + head * D, D, gn);
-                q.split(r.scale * 1.4426950408889634f);
-                uint32_t v[B::kWords] = {};
-#pragma unroll
-                for (int e = 0; e < A::kKS * A::kQP * 2; e++) v[e] = q.f[e / (A::kQP * 2)][e / 2 % A::kQP][e % 2];
-                v[A::kKS * A::kQP * 2] = __float_as_uint(q.undo0);
-                v[A::kKS * A::kQP * 2 + 1] = __float_as_uint(q.undo1);
-#pragma unroll
-                for (int e = 0; e < B::kWords / 4; e++)
-                  operands[(warp * (B::kWords / 4) + e) * 32 + lane] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                if (lane < 8) {
-                  const float lse = lane < gn ? r.lse[head + lane] : INFINITY;
-                  row_lse[warp * 8 + lane] = fabsf(lse) < INFINITY ? lse * 1.4426950408889634f : INFINITY;
-                }
-                if (lane == 0) row_len[warp] = r.len[i] <= cap ? r.len[i] : 0;
-              }
+              q.fetch(r.q + head * D, D, gn);
+              float lse0 = 2 * t < gn ? r.lse[head + 2 * t] : INFINITY, lse1 = 2 * t + 1 < gn ? r.lse[head + 2 * t + 1] : INFINITY;
+              lse0 = fabsf(lse0) < INFINITY ? lse0 * 1.4426950408889634f : INFINITY;  // (inf: no weights)
+              lse1 = fabsf(lse1) < INFINITY ? lse1 * 1.4426950408889634f : INFINITY;
+              q.split(r.scale * 1.4426950408889634f);
               copy_wait<0>();
-              __syncthreads();
-              for (uint32_t k1 = 0; k1 < min((uint32_t)W, n - k0); k1++) {
-                const uint32_t len = row_len[k1];
-                if (j0 >= len) continue;
-                uint32_t v[B::kWords];
+              __syncwarp();
 #pragma unroll
-                for (int e = 0; e < B::kWords / 4; e++)
-                  *reinterpret_cast<uint4*>(v + 4 * e) = operands[(k1 * (B::kWords / 4) + e) * 32 + lane];
-#pragma unroll
-                for (int e = 0; e < A::kKS * A::kQP * 2; e++) q.f[e / (A::kQP * 2)][e / 2 % A::kQP][e % 2] = v[e];
-                q.undo0 = __uint_as_float(v[A::kKS * A::kQP * 2]);
-                q.undo1 = __uint_as_float(v[A::kKS * A::kQP * 2 + 1]);
+              for (uint32_t u = 0; u < kTiles; u++) {
+                const uint32_t j = j0 + u * kTile;
+                if (j >= len) break;
                 float x[4];
-                q.scores(tile_a, x);
-                const float lse0 = row_lse[k1 * 8 + 2 * t], lse1 = row_lse[k1 * 8 + 2 * t + 1];
-                const bool in0 = j0 + g < len, in8 = j0 + g + 8 < len;
-                if (lse0 < INFINITY) {
-                  w0 += in0 ? pow2(x[0] - lse0) : 0.f;
-                  w8 += in8 ? pow2(x[2] - lse0) : 0.f;
-                }
-                if (lse1 < INFINITY) {
-                  w0 += in0 ? pow2(x[1] - lse1) : 0.f;
-                  w8 += in8 ? pow2(x[3] - lse1) : 0.f;
-                }
+                q.scores(tile_a + u * B::kTileBytes, x);
+                const bool in0 = j + g < len, in8 = j + g + 8 < len;
+                w0[u] += in0 && lse0 < INFINITY ? pow2(x[0] - lse0) : 0.f;
+                w8[u] += in8 && lse0 < INFINITY ? pow2(x[2] - lse0) : 0.f;
+                w0[u] += in0 && lse1 < INFINITY ? pow2(x[1] - lse1) : 0.f;
+                w8[u] += in8 && lse1 < INFINITY ? pow2(x[3] - lse1) : 0.f;
               }
             }
-          w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
-          w8 += __shfl_xor_sync(0xffffffffu, w8, 1);
-          w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
-          w8 += __shfl_xor_sync(0xffffffffu, w8, 2);
-          const uint32_t slot = j0 + g + 8 * t;
-          if (t < 2 && slot < longest) r.weights[((uint64_t)s * c.kvheads + h) * cap + slot] += t ? w8 : w0;
-          __syncwarp();  // (the tile is read)
+          }
+        copy_wait<0>();
+#pragma unroll
+        for (uint32_t u = 0; u < kTiles; u++) {
+          w0[u] += __shfl_xor_sync(0xffffffffu, w0[u], 1);
+          w8[u] += __shfl_xor_sync(0xffffffffu, w8[u], 1);
+          w0[u] += __shfl_xor_sync(0xffffffffu, w0[u], 2);
+          w8[u] += __shfl_xor_sync(0xffffffffu, w8[u], 2);
+          const uint32_t slot = j0 + u * kTile + g + 8 * t;
+          if (t < 2 && slot < longest) w[slot] = old[u] + (t ? w8[u] : w0[u]);
         }
-        __syncthreads();
+        __syncwarp();  // (the tiles are read)
       }
     }
+  }
 }
 
 // A weight's place in the order of eviction: larger weights have larger keys, NaN the smallest.
@@ -1164,30 +1086,21 @@ cudaError_t launch_paged_append(const PagedKV& c, const float* k, const float* v
 
 namespace {
 
-constexpr uint32_t kMaxAttSmem = 220 * 1024;
 
-template <class T, int DP, bool WEIGHTS, int W>
+template <class T, int DP, int W>
 cudaError_t att_prepare() {
-  using A = Att<T, DP>;
-  auto* f = k_paged_attention<T, DP, WEIGHTS, W>;
-  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       WEIGHTS ? (int)kMaxAttSmem : A::fixed(W));
+  auto* f = k_paged_attention<T, DP, W>;
+  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, Att<T, DP>::fixed(W));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
 }
 
 // A cluster of C blocks of W warps a (row, KV head).
-template <class T, int DP, bool WEIGHTS, int W>
-cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_t tiles, cudaStream_t st) {
+template <class T, int DP, int W>
+cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, cudaStream_t st) {
   using A = Att<T, DP>;
-  static_assert(A::fixed(W) <= (int)kMaxAttSmem, "shared memory of a block");
-  AttSplit sp{C, 0, 0, 0, false};
-  if (WEIGHTS) {
-    const uint32_t room = (kMaxAttSmem - A::fixed(W)) / (W * 512);
-    auto per_warp = [&] { return (tiles + W * sp.blocks - 1) / (W * sp.blocks); };
-    while (sp.blocks < (uint32_t)kMaxCluster && per_warp() > room) sp.blocks++;
-    sp.score_tiles = per_warp() < room ? per_warp() : room;
-  }
+  static_assert(A::fixed(W) <= 227 * 1024, "shared memory of a block");
+  AttSplit sp{C, 0, 0, false};
   // Where the blocks take two to three turns on the GPU, the short rows should be the last: 21 sequences of
   // 0..1531 positions in f32 29.5 -> 24.5 us, 64 of 130..4096 in bf16 60.5 -> 58.8, but 64 of 4096 each, where
   // it only delays the start, 100 -> 106; with more turns the end matters less than the start.
@@ -1199,7 +1112,7 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(r.rows * sp.blocks, c.kvheads);
   cfg.blockDim = dim3(W * 32);
-  cfg.dynamicSmemBytes = A::fixed(W) + sp.score_tiles * W * 512;
+  cfg.dynamicSmemBytes = A::fixed(W);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1207,7 +1120,7 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, WEIGHTS, W>, c, r, sp);
+  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, W>, c, r, sp);
 }
 
 // Blocks of a cluster, and warps of a block.  Where the largest clusters leave SMs to spare, as many as there
@@ -1217,7 +1130,7 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_
 // take 106 us with 8 blocks (768 in all), 118 with 6, 136 with 16.  Large clusters leave parts of a GPC
 // unused; where they would not all find room at once, clusters that do are better (32 units of 9000..32768
 // positions: 73 us with 12 blocks, 80 with 16, 88 with 8).
-template <class T, int DP, bool WEIGHTS>
+template <class T, int DP>
 cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   using A = Att<T, DP>;
   const uint32_t units = r.rows * c.kvheads, tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
@@ -1226,13 +1139,12 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
          (units * C < 148 || (units * C < 700 && tiles >= 12 * A::W * C)))
     C *= 2;
   if (C == (uint32_t)kMaxCluster && units > 384 / C) C = 384 / units > 8 ? 384 / units : 8;
-  // (blocks of two warps that keep many scores would be alone on their SM, so they had better be wide: 51
-  // sequences of 715..1276 positions, 24 heads of 192 in f32, 287 -> 182 us; with few tiles they are not)
-  const bool wide = (units * C <= 148 && tiles > A::W * C) || (WEIGHTS && A::W == 2 && tiles > 4 * A::W * C);
-  cudaError_t e = wide ? att_launch<T, DP, WEIGHTS, A::kWide>(c, r, C, tiles, st)
-                                                       : att_launch<T, DP, WEIGHTS, A::W>(c, r, C, tiles, st);
-  if (WEIGHTS && r.shared && e == cudaSuccess) {
-    k_paged_weights<T, DP><<<2 * 148, Give<T, DP>::W * 32, Give<T, DP>::kSmem + c.n_seqs * 4 + (c.n_seqs + 31) / 32 * 8, st>>>(c, r);
+  const bool wide = units * C <= 148 && tiles > A::W * C;
+  cudaError_t e = wide ? att_launch<T, DP, A::kWide>(c, r, C, st) : att_launch<T, DP, A::W>(c, r, C, st);
+  if (r.weights && e == cudaSuccess) {
+    using B = Give<T, DP>;
+    const uint32_t smem = B::kSmem + c.n_seqs * 4, per_sm = 225 * 1024 / (smem + 1024);
+    k_paged_weights<T, DP><<<148 * (per_sm > 4 ? 4 : per_sm), B::W * 32, smem, st>>>(c, r);
     e = cudaGetLastError();
   }
   return e;
@@ -1254,20 +1166,19 @@ struct AttLaunch {
   cudaStream_t st;
   template <class T, int DP>
   cudaError_t operator()() const {
-    return r.weights ? att_launch<T, DP, true>(c, r, st) : att_launch<T, DP, false>(c, r, st);
+    return att_launch<T, DP>(c, r, st);
   }
 };
 struct AttPrepare {
   template <class T, int DP>
   cudaError_t operator()() const {
     using A = Att<T, DP>;
-    cudaError_t e = att_prepare<T, DP, false, A::W>();
-    if (e == cudaSuccess) e = att_prepare<T, DP, false, A::kWide>();
-    if (e == cudaSuccess) e = att_prepare<T, DP, true, A::W>();
-    if (e == cudaSuccess) e = att_prepare<T, DP, true, A::kWide>();
+    static_assert(Give<T, DP>::kSmem + (int)kMaxWeightSeqs * 4 <= 227 * 1024, "shared memory of a block");
+    cudaError_t e = att_prepare<T, DP, A::W>();
+    if (e == cudaSuccess) e = att_prepare<T, DP, A::kWide>();
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(k_paged_weights<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               Give<T, DP>::kSmem + (int)kMaxSharedSeqs * 4 + (int)kMaxSharedSeqs / 4);
+                               Give<T, DP>::kSmem + (int)kMaxWeightSeqs * 4);
     return e;
   }
 };
