@@ -259,7 +259,8 @@ int qc_batch_ep_connect(qc_batch* b, const void* handles, const int* device_ids)
  * All arguments that are not sizes are DEVICE pointers on one device (pools, q, k, v and out 16-byte
  * aligned); the call runs on that device and on `stream` (a cudaStream_t of that device; NULL = its
  * default stream), allocates nothing, keeps nothing between calls and returns once the work is
- * enqueued, so it can be captured into a CUDA graph.  Errors: qc_last_error().  What lies on the device
+ * enqueued, so it can be captured into a CUDA graph (the first call on a device loads the kernels: make
+ * it before a capture).  Errors: qc_last_error().  What lies on the device
  * is checked there: a row of a sequence >= n_seqs (padding) is skipped and its outputs left as they
  * were; a length beyond max_pages * page or a page number >= n_pages among the slots a row uses makes
  * its results NaN (attention), or leaves the slot or the sequence as it was (append, evict).
@@ -289,8 +290,8 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
 /* Eviction by accumulated attention weight: of a sequence of len[s] > keep slots, every KV head keeps the
  * last `recent` slots and, of the others, the keep - recent with the largest weights (equal weights: the
  * lower slot; NaN counts as the smallest).  Their rows and weights move, in their order, to slots
- * 0..keep-1 of the pages dst_table[s] ([n_seqs][max_pages]; NULL: in place) and to weights_out (may be
- * weights).  kept ([n_seqs][kvheads][keep]) receives the slots' old numbers (0xffffffff behind the last
+ * 0..keep-1 of the pages dst_table[s] ([n_seqs][max_pages]; NULL: in place) and to weights_out (weights
+ * itself, or apart from it).  kept ([n_seqs][kvheads][keep]) receives the slots' old numbers (0xffffffff behind the last
  * one), new_len (may be len) min(len, keep).  A sequence within keep keeps all slots (and is copied
  * where dst_table names other pages).  A page of dst_table belongs to one sequence and is not read by
  * this call; in place (dst_table NULL or the table itself) a sequence's pages are its own. */

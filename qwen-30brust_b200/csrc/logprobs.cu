@@ -78,8 +78,13 @@ __device__ __forceinline__ uint32_t lp_cluster_addr(const void* p, uint32_t rank
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void lp_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void lp_cluster_arrive() {
+  __syncwarp();  // (the barrier wants a warp's threads together)
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void lp_cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Shared memory; behind it the chunks on their way, later the block's candidates.
@@ -196,6 +201,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(LogprobArgs a, uint3
   uint8_t* const behind = lp_smem + sizeof(LpShared);
   const uint32_t C = 1u << logc, rank = blockIdx.x & (C - 1), row = blockIdx.x >> logc, tid = threadIdx.x;
   const uint32_t warp = tid / 32, lane = tid % 32, n = a.n, k = a.top;
+  lp_cluster_arrive();  // this block runs: it may be written to
   const float* x = a.logits + (uint64_t)(a.src ? a.src[row] : row) * a.stride;
   // 16-byte pieces of the row; piece 0 starts at the boundary at or before x[0]
   const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(x) / 4 % 4);
@@ -407,6 +413,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(LogprobArgs a, uint3
     have = min(all, k);
   }
   // the block's, to every block
+  lp_cluster_wait();  // (they all run)
   if (tid < C) {
     Part part = sh.warp_part[0];
 #pragma unroll
@@ -423,7 +430,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(LogprobArgs a, uint3
                  : "memory");
   }
   if (tid < kMaxTop) sh.rank[tid] = tid;
-  lp_cluster_sync();
+  lp_cluster_arrive();
+  lp_cluster_wait();
   Part all = sh.in_part[0];
   for (uint32_t c = 1; c < C; c++) all = join(all, sh.in_part[c]);
   const float qnan = __int_as_float(0x7fc00000), lg = log1pf(all.l);

@@ -177,8 +177,17 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[P])
   }
 }
 
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();  // (the barrier wants a warp's threads together)
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 // This block's shared address `a` in block `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t a, uint32_t rank) {
@@ -418,6 +427,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
   }
   const uint32_t s = r.seq ? r.seq[i] : i, len = r.len[i];
   if (s >= c.n_seqs) return;  // (the whole cluster)
+  cluster_arrive();  // this block runs, and in_o and in_m may be written
   const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
   // Where pages hold whole runs of 8 positions a lane copies its part of a run with one address; else every
   // position has its own page and its lanes ask the lane that looked it up.  64 sequences of 4096
@@ -426,8 +436,6 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
   const uint32_t step = C * W * kTile, gw = rank * W + warp;
   const uint32_t ahead = runs ? lane / 16 * 8 : lane % kTile;  // the position of a tile this lane looks up
   const uint32_t page0 = (gw * kTile + ahead) / c.page, slot0 = (gw * kTile + ahead) % c.page;
-  bool again = false;
-
   const bool too_long = len > cap;
   const uint32_t tiles = too_long ? 0 : (len + kTile - 1) / kTile;
   const uint32_t mine_n = tiles > gw ? (tiles - gw + C * W - 1) / (C * W) : 0;  // this warp's tiles
@@ -583,9 +591,8 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
       mine[8 * A::kO + 2 * t] = l0 * f0;
       mine[8 * A::kO + 2 * t + 1] = l1 * f1;
     }
-    if (again) cluster_sync();  // the other blocks have read what was sent for the previous turn
-    else __syncthreads();
-    again = true;
+    __syncthreads();
+    cluster_wait();  // the other blocks run, and have read what was sent for the previous turn
     // what they add up to goes to the blocks of the cluster: a share of O to each, maxima and sums to all
     auto part = [&](uint32_t w) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage); };
     const uint32_t share = (2 * DP + C - 1) / C;  // 16-byte pieces of O of one block (the last may have fewer)
@@ -646,6 +653,7 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
           make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
       if (d == 0 && r.lse) r.lse[row_head + hh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
+    if (g0 + 8 < G) cluster_arrive();
   }
 }
 
@@ -859,6 +867,7 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
     }
     return;
   }
+  if (C > 1) cluster_sync();  // (the blocks of the cluster run: they may be written to)
   const uint32_t old = n - e.recent, want = e.keep - e.recent;
   // the sum of a and of b over the warps before this one, and over all (a, b: the same in all lanes)
   auto scan = [&](uint32_t& a, uint32_t& b, uint32_t& all_a, uint32_t& all_b) {
@@ -1188,6 +1197,11 @@ struct AttPrepare {
 // Once per device, before launch_paged_attention.
 cudaError_t paged_prepare() {
   cudaError_t e = cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelHold * 4);
+  cudaFuncAttributes loaded;  // (a kernel is loaded when it is first asked about: not in a capture)
+  for (uint32_t kind : {(uint32_t)F32, (uint32_t)F16, (uint32_t)BF16}) {
+    if (e == cudaSuccess) QC_BY_KIND(kind, e = cudaFuncGetAttributes(&loaded, k_paged_append<T>));
+    if (e == cudaSuccess) QC_BY_KIND(kind, e = cudaFuncGetAttributes(&loaded, k_evict_move<T>));
+  }
   for (uint32_t D : {32u, 64u, 96u, 128u, 192u, 256u}) {
     if (e == cudaSuccess) e = by_width<float>(D, AttPrepare{});
     if (e == cudaSuccess) e = by_width<__half>(D, AttPrepare{});
