@@ -1,9 +1,10 @@
 """qc_logprobs against log-softmax in 64 bits.
 
-Bounds: d = x - max is one f32 rounding (2^-24 |d|), log1p of a sum whose relative error is at most
-2^-24 times the additions in a row (a few hundred at the sizes here, pairwise joined) plus the
-roundings of exp (2 ulp): 1e-4 of one nat would be far outside.  Log probabilities are held to
-2^-21 |d| + 2e-6 (l's relative error), the entropy to 4e-6 (1 + H)."""
+Bounds: d = x - max is rounded once, 2^-24 |d|; the sum's terms carry exp's 2 ulp and the rounding of d
+times log2 e, 2^-24 |d|, each its own, so that the sum is good to about 1e-6 with the few hundred
+additions in a row that a lane makes.  A log probability is held to 2^-21 |d| + 2e-6 of it, or of one
+where it is larger; the entropy to 5e-6 of it.
+"""
 import math
 
 import pytest

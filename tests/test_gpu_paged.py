@@ -407,3 +407,90 @@ def test_no_rows_and_host_pointers(cuda_engine, torch_cuda):
     with pytest.raises(cuda_engine.QwenCudaError, match="len is not device memory"):
         h.attention(ptr(q), 4, 1, ptr(ln), ptr(out))
     assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("kind,heads,kvheads,D,page,rows,hi,pad", [
+    ("bf16", 32, 4, 128, 16, 64, 900, 0),   # more blocks than fit at once: the longest rows first
+    ("f16", 32, 4, 128, 16, 8, 9000, 0),    # clusters of other than a power of two
+    ("f32", 6, 2, 64, 24, 130, 300, 5),     # more rows than are sorted
+    ("bf16", 10, 1, 32, 3, 700, 70, 1),
+    ("f16", 24, 8, 256, 128, 40, 700, 2),
+])
+def test_many_rows(cuda_engine, torch_cuda, kind, heads, kvheads, D, page, rows, hi, pad):
+    """Lengths all over the range, empty ones among them, padding behind; with and without weights."""
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, hi + 1, (rows,), generator=g).tolist()
+    lens[0], lens[-1], lens[rows // 2] = hi, 0, 1
+    cache = Cache(kind, kvheads, D, page, lens, seed=2)
+    q = torch.randn(rows + pad, heads, D, generator=g).cuda()
+    seq = torch.randperm(rows, generator=g).tolist()
+    real = [lens[s] for s in seq]
+    weights = torch.rand(rows, kvheads, cache.cap, generator=g).cuda()
+    before = weights.clone()
+    out, lse = run_attention(cuda_engine, cache, q, seq + [-1] * pad, real + [0] * pad, weights=weights)
+    check_attention(cache, q[:rows], seq, real, out[:rows], lse[:rows], weights=weights, before=before)
+    assert bool((out[rows:] == 7).all()) and bool((lse[rows:] == 7).all())
+    again, _ = run_attention(cuda_engine, cache, q, seq + [-1] * pad, real + [0] * pad)
+    assert torch.equal(again, out)
+
+
+def test_many_rows_of_one_sequence_give_their_weights_in_any_call(cuda_engine, torch_cuda):
+    """A prompt's 150 tokens in one call, and each in a call of its own: the same outputs, and weights that
+    differ by the additions' roundings only (one a call: 150 half steps)."""
+    cache = Cache("f16", 2, 64, 16, [400, 30], seed=5)
+    q = torch.randn(150, 8, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    seq, lens = [0] * 150, list(range(251, 401))
+    one, many = (torch.zeros(2, 2, cache.cap, device="cuda") for _ in range(2))
+    out, _ = run_attention(cuda_engine, cache, q, seq, lens, weights=one)
+    for i in range(150):
+        row, _ = run_attention(cuda_engine, cache, q[i:i + 1].contiguous(), [0], [lens[i]], weights=many)
+        assert torch.allclose(row[0], out[i], rtol=0, atol=2e-6)
+    assert bool(((one - many).abs() <= 1e-5 * many.abs() + 1e-9).all())
+    assert bool((one[1] == 0).all())
+
+
+def test_a_slot_named_twice_holds_one_of_the_rows(cuda_engine, torch_cuda):
+    """Rows of a call have different slots; where they do not, every value is one of theirs."""
+    cache = Cache("bf16", 2, 64, 16, [5], cap=32, seed=1)
+    k, v = torch.ones(4, 2, 64, device="cuda"), torch.ones(4, 2, 64, device="cuda")
+    k *= torch.arange(1, 5, device="cuda")[:, None, None]
+    seq, pos = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.full((4,), 7, dtype=torch.int32, device="cuda")
+    cache.handle(cuda_engine).append(ptr(k), ptr(v), 4, ptr(pos), seq_ptr=ptr(seq))
+    torch.cuda.synchronize()
+    got = cache.rows(0, 8)[7].float()
+    assert bool(((got >= 1) & (got <= 4) & (got == got.round())).all())
+
+
+@pytest.mark.parametrize("S,n,keep,recent", [(150, 41500, 30001, 77), (1, 400003, 123457, 1000)])
+def test_evict_of_more_slots_than_are_held(cuda_engine, torch_cuda, S, n, keep, recent):
+    """Sequences whose weights do not fit the selection's shared memory, alone and with many short ones."""
+    lens = [n] + [100] * (S - 1)
+    cache = Cache("f32", 1, 4, 64, lens, seed=6)
+    w = torch.floor(torch.rand(S, 1, cache.cap, generator=torch.Generator().manual_seed(1)) * 50000)  # ties
+    weights, lens_d = w.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kept = torch.zeros(S, 1, keep, dtype=torch.int32, device="cuda")
+    old = cache.rows(0, n, "v").clone()
+    cache.handle(cuda_engine).evict(ptr(weights), ptr(lens_d), keep, recent, ptr(kept), ptr(lens_d))
+    torch.cuda.synchronize()
+    want = torch.tensor(evict64(w[0, 0], n, keep, recent))
+    assert lens_d.tolist() == [keep] + [100] * (S - 1)
+    assert torch.equal(kept[0, 0].long().cpu(), want)
+    assert torch.equal(weights[0, 0, :keep].cpu(), w[0, 0][want])
+    assert torch.equal(cache.rows(0, keep, "v")[:, 0], old[want.cuda(), 0])
+
+
+def test_calls_at_once_on_two_streams(cuda_engine, torch_cuda):
+    """Calls on different caches from two streams, many times over, give what they give alone."""
+    caches = [Cache(kind, 4, 128, 16, [300 + 50 * i for i in range(12)], seed=i) for i, kind in enumerate(("bf16", "f16"))]
+    g = torch.Generator().manual_seed(1)
+    qs = [torch.randn(12, 32, 128, generator=g).cuda() for _ in caches]
+    alone = [run_attention(cuda_engine, c, q, None, c.lens)[0] for c, q in zip(caches, qs)]
+    streams = [torch.cuda.Stream() for _ in caches]
+    outs = [torch.zeros_like(a) for a in alone]
+    lens = [torch.tensor(c.lens, dtype=torch.int32, device="cuda") for c in caches]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, q, o, ln, st in zip(caches, qs, outs, lens, streams):
+            c.handle(cuda_engine).attention(ptr(q), 32, 12, ptr(ln), ptr(o), stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, o) for a, o in zip(alone, outs))
