@@ -1090,6 +1090,7 @@ struct qc_batch {
     float* d_lse = nullptr;                                 // [cap][heads], with eviction
     uint32_t *d_lens = nullptr, *d_kept = nullptr;          // [2][seq]; [seq][kv head][kept_n]
     uint64_t kept_n = 0;
+    bool shared = false;                                    // nearly all of a pass's neighbouring rows are of one sequence
     std::vector<uint32_t> table, cached, unused;
   };
   std::unique_ptr<Pages> pg;
@@ -1489,7 +1490,8 @@ struct qc_batch {
       if (pg) {
         const uint32_t *seq = pg->d_rows, *slot = seq + cap, *len = slot + cap;
         QC_CK(qc::launch_paged_append(pages_of(l), d_k, d_v, T, seq, slot, weights_of(l), s));
-        const qc::PagedRows r{d_q, c.heads, T, seq, len, 1.f / std::sqrt((float)c.head_dim), d_a, pg->d_lse, weights_of(l)};
+        const qc::PagedRows r{d_q, c.heads, T, seq, len, 1.f / std::sqrt((float)c.head_dim), d_a, pg->d_lse, weights_of(l),
+                              pg->shared};
         QC_CK(qc::launch_paged_attention(pages_of(l), r, s));
       } else {
         qc::launch_batch_attention(ba, l, d_q, d_a, T, s);
@@ -1598,12 +1600,15 @@ struct qc_batch {
   // The cache rows of a pass of T tokens (paged cache): cached[q] further slots, taken as they come.
   void stage_rows(const qc::BatchTok* tk, uint32_t T, std::vector<uint32_t>& rows) {
     rows.assign(3ull * cap, 0);
+    uint32_t same = 0;
     for (uint32_t i = 0; i < T; i++) {
+      same += i && tk[i].seq == tk[i - 1].seq;
       const uint32_t q = tk[i].seq, slot = pg->cached[q]++;
       rows[i] = q;
       rows[cap + i] = slot;
       rows[2 * cap + i] = slot + 1;
     }
+    pg->shared = 16 * same >= 15 * T;
     QC_CK(cudaMemcpyAsync(pg->d_rows, rows.data(), rows.size() * 4, cudaMemcpyHostToDevice, e->stream));
   }
 
@@ -2440,7 +2445,8 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     at.add(lse, "lse");
     at.add(weights, "weights");
     at.enter();
-    qc::PagedRows r{q, heads, rows, seq, len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale, out, lse, weights};
+    qc::PagedRows r{q, heads, rows, seq, len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale, out, lse, weights,
+                    rows / 16 >= n_seqs};
     QC_CK(qc::launch_paged_attention(c, r, static_cast<cudaStream_t>(stream)));
   });
 }

@@ -87,6 +87,11 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __
 // units, whose accumulators truncate.  Queries of one KV head share K and V; more than 8 heads take
 // another turn over the sequence, 8 at a time.
 //
+// Neighbouring rows of one sequence (prompts) are taken R units of 8 (row, head) columns at a time, their q's
+// planes in shared memory: K and V come from L2 once for up to 8 R columns, and a unit's products fill the waits
+// of another's.  512 rows of 4096 positions, 32/4 heads of 128 bf16: 361 us, the matrix units busy about half
+// the time (48 products a tile and unit); a row at a time 449.
+//
 // The warps' (maximum, sum, O) are joined in shared memory, the blocks' through the cluster's
 // distributed shared memory in a fixed order: no workspace, no atomics, the same bits every time.
 
@@ -106,8 +111,17 @@ struct Att {
   static constexpr int NS = kFit > 4 ? 4 : kFit < 2 ? 2 : kFit;
   static constexpr int kWide = 200 * 1024 / (NS * kStage) > 8 ? 8 : 200 * 1024 / (NS * kStage);  // one block an SM
   static constexpr int kO = DP + 4;                                // floats between two heads' O in a warp's part
-  // ring of w warps; this block's share of every block's O; every block's 8 maxima and 8 sums; the warps' maxima
-  static constexpr int fixed(int w) { return w * NS * kStage + (2 * DP + kMaxCluster) * 16 + kMaxCluster * 16 * 4 + w * 8 * 4; }
+  static constexpr int kShared = DP <= 128 ? 4 : 2;                // units of a block that shares tiles among rows
+  static constexpr int kPlanes = kKS * 32 * kQP * 2;               // words of a unit's q
+  // this block's share of every block's O; of several units, their q before
+  static constexpr int space(int units) {
+    const int o = units * (2 * DP + kMaxCluster) * 16, q = units > 1 ? units * kPlanes * 4 : 0;
+    return o > q ? o : q;
+  }
+  // ring of w warps; space; every block's maxima and sums; the warps' maxima; columns' lengths, factors; bad slots
+  static constexpr int fixed(int w, int units) {
+    return w * NS * kStage + space(units) + units * kMaxCluster * 16 * 4 + w * units * 8 * 4 + (units > 1 ? units * 64 + w * 4 : 0);
+  }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -214,6 +228,57 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
+// Scores (times log2 e, and q's scaling) of a K tile and of n <= R units of 8 columns (queries): s[u][0], s[u][1]
+// for position lane / 4 and columns 2 (lane % 4), + 1; s[u][2], s[u][3] for position lane / 4 + 8.  frag(u, k, b):
+// the planes of q^T of unit u, step k.  All: n = R; without a test at every unit the compiler interleaves their
+// products (512 rows of 4096 positions, 32/4 heads of 128 bf16: 361 us against 489).
+template <class T, int DP, int R, bool All, class F>
+__device__ __forceinline__ void scores_of(uint32_t ktile, uint32_t n, F&& frag, float (&s)[R][4]) {
+  using A = Att<T, DP>;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t a0 = ktile + ((lane / 8 % 2) * 8 + lane % 8) * A::kRow + (lane / 16) * 16;
+  float c[R][A::kF32 ? 3 : A::kQP][4];
+#pragma unroll
+  for (auto& u : c)
+#pragma unroll
+    for (auto& x : u) x[0] = x[1] = x[2] = x[3] = 0.f;
+#pragma unroll
+  for (int k = 0; k < A::kKS; k++) {
+    uint32_t a[4], b[A::kQP][2];
+    ldsm4(a, a0 + k * 32);
+    if constexpr (A::kF32) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(a[i]), hi[i], lo[i]);
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        if (!All && u >= n) break;
+        frag(u, k, b);
+        mma8(c[u][0], hi, b[0][0], b[0][1]);
+        mma8(c[u][1], hi, b[1][0], b[1][1]);
+        mma8(c[u][2], lo, b[0][0], b[0][1]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        if (!All && u >= n) break;
+        frag(u, k, b);
+#pragma unroll
+        for (int p = 0; p < A::kQP; p++) mma16<T>(c[u][p], a, b[p][0], b[p][1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < R; u++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (A::kF32 || A::kQP == 3)
+        s[u][i] = c[u][0][i] + (c[u][1][i] + c[u][2][i]);
+      else
+        s[u][i] = c[u][0][i] + c[u][1][i];
+    }
+}
+
 // One warp's query operand: the B fragments of q^T for 8 heads, and the factor that undoes q's scaling
 // for the two heads whose scores this lane holds.
 template <class T, int DP>
@@ -221,23 +286,22 @@ struct Query {
   using A = Att<T, DP>;
   float raw[A::kKS][A::kF32 ? 2 : 4];
   uint32_t f[A::kKS][A::kQP][2];
-  float undo0, undo1;
+  float undo0, undo1, undo;  // (undo: of column lane / 4)
 
-  // Starts reading q (head 0 of the group); heads >= G and values >= D are zero.
-  __device__ __forceinline__ void fetch(const float* q, uint32_t D, uint32_t G) {
-    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
-    const float* qr = q + (uint64_t)g * D;
+  // Starts reading q, column lane / 4 at qr; columns that are not real and values >= D are zero.
+  __device__ __forceinline__ void fetch(const float* qr, uint32_t D, bool real) {
+    const uint32_t t = threadIdx.x & 3;
 #pragma unroll
     for (int k = 0; k < A::kKS; k++)
 #pragma unroll
       for (int b = 0; b < 2; b++) {
         if constexpr (A::kF32) {
           const uint32_t d = k * 8 + b * 4 + t;
-          raw[k][b] = g < G && d < D ? qr[d] : 0.f;
+          raw[k][b] = real && d < D ? qr[d] : 0.f;
         } else {
           const uint32_t d = k * 16 + b * 8 + 2 * t;
           float2 x = make_float2(0.f, 0.f);
-          if (g < G && d < D) x = *reinterpret_cast<const float2*>(qr + d);
+          if (real && d < D) x = *reinterpret_cast<const float2*>(qr + d);
           raw[k][2 * b] = x.x;
           raw[k][2 * b + 1] = x.y;
         }
@@ -246,7 +310,7 @@ struct Query {
   // Splits q times factor (scale log2 e) into planes.
   __device__ __forceinline__ void split(float factor) {
     const uint32_t t = threadIdx.x & 3;
-    undo0 = undo1 = 1.f;
+    undo0 = undo1 = undo = 1.f;
     if constexpr (A::kF32) {
 #pragma unroll
       for (int k = 0; k < A::kKS; k++) {
@@ -267,9 +331,9 @@ struct Query {
         int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
         e = mx == 0.f || mx > FLT_MAX ? 0 : e > 120 ? 120 : e;
         up = __uint_as_float((uint32_t)(127 + e) << 23);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        undo0 = __shfl_sync(0xffffffffu, down, 8 * t);
-        undo1 = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+        undo = __uint_as_float((uint32_t)(127 - e) << 23);
+        undo0 = __shfl_sync(0xffffffffu, undo, 8 * t);
+        undo1 = __shfl_sync(0xffffffffu, undo, 8 * t + 4);
       }
 #pragma unroll
       for (int k = 0; k < A::kKS; k++) {
@@ -287,130 +351,130 @@ struct Query {
     }
   }
 
-  // Scores (times log2 e) of a K tile: s[0], s[1] for position lane / 4 and heads 2 (lane % 4), + 1;
-  // s[2], s[3] for position lane / 4 + 8.
   __device__ __forceinline__ void scores(uint32_t ktile, float (&s)[4]) const {
-    const uint32_t lane = threadIdx.x & 31;
-    const uint32_t a0 = ktile + ((lane / 8 % 2) * 8 + lane % 8) * A::kRow + (lane / 16) * 16;
-    float c[A::kF32 ? 3 : A::kQP][4];
+    float x[1][4];
+    scores_of<T, DP, 1, true>(ktile, 1, [&](int, int k, uint32_t (&b)[A::kQP][2]) {
 #pragma unroll
-    for (auto& x : c) x[0] = x[1] = x[2] = x[3] = 0.f;
-#pragma unroll
-    for (int k = 0; k < A::kKS; k++) {
-      uint32_t a[4];
-      ldsm4(a, a0 + k * 32);
-      if constexpr (A::kF32) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(a[i]), hi[i], lo[i]);
-        mma8(c[0], hi, f[k][0][0], f[k][0][1]);
-        mma8(c[1], hi, f[k][1][0], f[k][1][1]);
-        mma8(c[2], lo, f[k][0][0], f[k][0][1]);
-      } else {
-#pragma unroll
-        for (int p = 0; p < A::kQP; p++) mma16<T>(c[p], a, f[k][p][0], f[k][p][1]);
+      for (int p = 0; p < A::kQP; p++) {
+        b[p][0] = f[k][p][0];
+        b[p][1] = f[k][p][1];
       }
-    }
+    }, x);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float x = c[0][i];
-      if constexpr (A::kF32 || A::kQP == 3)
-        x += c[1][i] + c[2][i];
-      else
-        x += c[1][i];
-      s[i] = x * (i % 2 ? undo1 : undo0);
-    }
+    for (int i = 0; i < 4; i++) s[i] = x[0][i] * (i % 2 ? undo1 : undo0);
   }
 };
 
-// O^T += V^T P^T for one tile; p as Query::scores lays its scores out.
-template <class T, int DP>
-__device__ __forceinline__ void add_values(uint32_t vtile, const float (&p)[4], float (&o)[DP / 16][4]) {
+// O^T += V^T P^T for one tile and n <= R units; p as scores_of lays its scores out.
+template <class T, int DP, int R, bool All>
+__device__ __forceinline__ void add_values(uint32_t vtile, uint32_t n, const float (&p)[R][4], float (&o)[R][DP / 16][4]) {
   using A = Att<T, DP>;
   const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
   if constexpr (A::kF32) {
     // k index i of a step of 8 positions stands for position 2 i (i < 4) or 2 (i - 4) + 1: the reads of V
     // then fall on 32 different banks
-    uint32_t hi[2][2], lo[2][2];
+    uint32_t hi[R][2][2], lo[R][2][2];
 #pragma unroll
-    for (int st = 0; st < 2; st++)
+    for (int u = 0; u < R; u++)
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        const uint32_t from = (2 * t + b) * 4 + g / 2;
-        const float x = __shfl_sync(0xffffffffu, p[2 * st], from), y = __shfl_sync(0xffffffffu, p[2 * st + 1], from);
-        split_tf32(g % 2 ? y : x, hi[st][b], lo[st][b]);
-      }
+      for (int st = 0; st < 2; st++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const uint32_t from = (2 * t + b) * 4 + g / 2;
+          const float x = __shfl_sync(0xffffffffu, p[u][2 * st], from), y = __shfl_sync(0xffffffffu, p[u][2 * st + 1], from);
+          split_tf32(g % 2 ? y : x, hi[u][st][b], lo[u][st][b]);
+        }
 #pragma unroll
     for (int m = 0; m < DP / 16; m++) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t ah[2][4], al[2][4];
 #pragma unroll
-      for (int st = 0; st < 2; st++) {
-        uint32_t ah[4], al[4];
+      for (int st = 0; st < 2; st++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           float x;
           const uint32_t a = vtile + (st * 8 + 2 * t + i / 2) * A::kRow + (m * 16 + g + (i % 2) * 8) * 4;
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(a) : "memory");
-          split_tf32(x, ah[i], al[i]);
+          split_tf32(x, ah[st][i], al[st][i]);
         }
-        mma8(c, al, hi[st][0], hi[st][1]);
-        mma8(c, ah, lo[st][0], lo[st][1]);
-        mma8(c, ah, hi[st][0], hi[st][1]);
-      }
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[m][i] += c[i];
+      for (int u = 0; u < R; u++) {
+        if (!All && u >= n) break;
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+          mma8(c, al[st], hi[u][st][0], hi[u][st][1]);
+          mma8(c, ah[st], lo[u][st][0], lo[u][st][1]);
+          mma8(c, ah[st], hi[u][st][0], hi[u][st][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[u][m][i] += c[i];
+      }
     }
   } else {
-    uint32_t lo8[A::kQP], hi8[A::kQP];
+    uint32_t lo8[R][A::kQP], hi8[R][A::kQP];
     const float up = __is_same(T, __half) ? 16384.f : 1.f;  // (undone with the final division)
-    split_pair<T, A::kQP>(p[0] * up, p[1] * up, lo8);
-    split_pair<T, A::kQP>(p[2] * up, p[3] * up, hi8);
 #pragma unroll
-    for (int q = 0; q < A::kQP; q++) {
-      lo8[q] = transpose8(lo8[q]);
-      hi8[q] = transpose8(hi8[q]);
+    for (int u = 0; u < R; u++) {
+      split_pair<T, A::kQP>(p[u][0] * up, p[u][1] * up, lo8[u]);
+      split_pair<T, A::kQP>(p[u][2] * up, p[u][3] * up, hi8[u]);
+#pragma unroll
+      for (int q = 0; q < A::kQP; q++) {
+        lo8[u][q] = transpose8(lo8[u][q]);
+        hi8[u][q] = transpose8(hi8[u][q]);
+      }
     }
     const uint32_t a0 = vtile + ((lane / 16) * 8 + lane % 8) * A::kRow + (lane / 8 % 2) * 16;
 #pragma unroll
     for (int m = 0; m < DP / 16; m++) {
       uint32_t a[4];
       ldsm4_t(a, a0 + m * 32);
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = A::kQP - 1; q >= 0; q--) mma16<T>(c, a, lo8[q], hi8[q]);
+      for (int u = 0; u < R; u++) {
+        if (!All && u >= n) break;
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[m][i] += c[i];
+        for (int q = A::kQP - 1; q >= 0; q--) mma16<T>(c, a, lo8[u][q], hi8[u][q]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[u][m][i] += c[i];
+      }
     }
   }
 }
 
 // How a launch splits a sequence: the blocks of a cluster; a warp's next tile lies step_pages pages and
-// step_slots slots further; whether the longest rows come first.
+// step_slots slots further; the rows of a group; whether the longest come first.
 struct AttSplit {
-  uint32_t blocks, step_pages, step_slots;
+  uint32_t blocks, step_pages, step_slots, rows;
   bool longest_first;
 };
 constexpr uint32_t kMaxSorted = 128;  // rows
 static_assert(kMaxSorted < kMaxCluster * 16, "lengths are sorted where the maxima and sums come later");
 
-template <class T, int DP, int W>
-__global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 : 1)
+template <class T, int DP, int W, int R>
+__global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <= 75 * 1024 ? 3 : 1)
     k_paged_attention(PagedKV c, PagedRows r, AttSplit sp) {
   using A = Att<T, DP>;
   constexpr int NS = A::NS;
+  constexpr int kPart = 8 * A::kO + 8;  // floats of a unit's O and sums
+  static_assert(R * kPart * 4 <= NS * A::kStage, "a warp's part lies in its ring");
   extern __shared__ __align__(16) uint8_t sm[];
-  float* const in_o = reinterpret_cast<float*>(sm + W * NS * A::kStage);  // [C][8 DP / C]: this block's share of every block's O
-  float* const in_m = in_o + 8 * DP + 4 * kMaxCluster;                            // [C][16]: every block's maxima, sums
-  float* const warp_m = in_m + kMaxCluster * 16;                // [W][8]
+  uint8_t* const space = sm + W * NS * A::kStage;
+  float* const in_o = reinterpret_cast<float*>(space);                  // [R][C][8 DP / C]: this block's share of every block's O
+  uint32_t* const planes = reinterpret_cast<uint32_t*>(space);          // R > 1, before: [R][kPlanes], the units' q
+  float* const in_m = reinterpret_cast<float*>(space + A::space(R));    // [R][C][16]: every block's maxima, sums
+  float* const warp_m = in_m + R * kMaxCluster * 16;                    // [W][R][8]
+  uint32_t* const col_len = reinterpret_cast<uint32_t*>(warp_m + W * R * 8);  // R > 1: [R][8]; kNoSlot: beyond the cache
+  float* const col_undo = reinterpret_cast<float*>(col_len + R * 8);          // R > 1: [R][8]
+  uint32_t* const warp_bad = col_len + R * 16;                                // R > 1: [W] first slot of an invalid page
   const uint32_t C = sp.blocks, h = blockIdx.y;
-  uint32_t rank, i;  // (the row)
+  uint32_t rank, first;  // (the row, or the rows' place among the clusters)
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm("mov.u32 %0, %%clusterid.x;" : "=r"(i));
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(first));
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t D = c.D, G = r.heads / c.kvheads, cap = c.max_pages * c.page, chunks = D * (uint32_t)sizeof(T) / 16;
   uint8_t* const ring = sm + warp * NS * A::kStage;
   const uint32_t ring_a = smem_addr(ring);
-  if (sp.longest_first) {  // the row of rank i among the lengths
+  if (R == 1 && sp.longest_first) {  // the row of rank `first` among the lengths
     uint32_t* const lens = reinterpret_cast<uint32_t*>(in_m);
     for (uint32_t k = tid; k < r.rows; k += W * 32) lens[k] = r.len[k];
     __syncthreads();
@@ -419,16 +483,21 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
       uint32_t before = 0;
 #pragma unroll 8
       for (uint32_t j = 0; j < r.rows; j++) before += lens[j] > n || (lens[j] == n && j < k);
-      if (before == i) lens[kMaxSorted] = k;
+      if (before == first) lens[kMaxSorted] = k;
     }
     __syncthreads();
-    i = lens[kMaxSorted];
+    first = lens[kMaxSorted];
     __syncthreads();  // (in_m is the cluster's from here on)
   }
-  const uint32_t s = r.seq ? r.seq[i] : i, len = r.len[i];
+  // Rows of a group (sp.rows of them) are computed together where all are of one sequence (R > 1), each by itself
+  // where they are not (R = 1); the other kernel's blocks leave.
+  const uint32_t i = R > 1 ? first * sp.rows : first, group = R > 1 ? i : i - i % sp.rows;
+  const uint32_t nr = R > 1 ? min(sp.rows, r.rows - i) : 1, s = r.seq ? r.seq[i] : i;
   if (s >= c.n_seqs) return;  // (the whole cluster)
-  cluster_arrive();  // this block runs, and in_o and in_m may be written
-  const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
+  if (sp.rows > 1) {
+    const bool other = lane < sp.rows && group + lane < r.rows && (r.seq ? r.seq[group + lane] : group + lane) != s;
+    if (__any_sync(0xffffffffu, other) == (R > 1)) return;
+  }
   // Where pages hold whole runs of 8 positions a lane copies its part of a run with one address; else every
   // position has its own page and its lanes ask the lane that looked it up.  64 sequences of 4096
   // positions in bf16: 100 us with pages of 16 slots (runs), 105 with pages of 250.
@@ -436,24 +505,49 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
   const uint32_t step = C * W * kTile, gw = rank * W + warp;
   const uint32_t ahead = runs ? lane / 16 * 8 : lane % kTile;  // the position of a tile this lane looks up
   const uint32_t page0 = (gw * kTile + ahead) / c.page, slot0 = (gw * kTile + ahead) % c.page;
-  const bool too_long = len > cap;
-  const uint32_t tiles = too_long ? 0 : (len + kTile - 1) / kTile;
-  const uint32_t mine_n = tiles > gw ? (tiles - gw + C * W - 1) / (C * W) : 0;  // this warp's tiles
-  for (uint32_t g0 = 0; g0 < G; g0 += 8) {
-    const uint32_t gn = min(8u, G - g0);
-    bool bad = false;
+  const uint32_t* const pages = c.table + (uint64_t)s * c.max_pages;
+  const uint32_t columns = nr * G;  // column x: row i + x / G, head x % G of the KV head's
+  for (uint32_t x0 = 0; x0 < columns; x0 += 8 * R) {
+    const uint32_t units = R > 1 ? min((uint32_t)R, (columns - x0 + 7) / 8) : 1;
+    auto column = [&](uint32_t x) {  // row of q, out and lse
+      return R > 1 ? (uint64_t)(i + x / G) * r.heads + h * G + x % G : (uint64_t)i * r.heads + h * G + x;
+    };
     Query<T, DP> q;
-    q.fetch(r.q + ((uint64_t)i * r.heads + h * G + g0) * D, D, gn);
+    bool bad = false;
+    uint32_t first_bad = kNoSlot, len, shortest = 0;
+    if constexpr (R == 1) {
+      cluster_arrive();  // this block runs, and in_o and in_m may be written
+      len = r.len[i];
+      q.fetch(r.q + column(x0 + g) * D, D, x0 + g < columns);
+      bad = len > cap;
+      if (bad) len = 0;
+    } else {
+      __syncthreads();  // (the last turn's results are read)
+      if (tid < R * 8) {
+        const uint32_t n = x0 + tid < columns ? r.len[i + (x0 + tid) / G] : 0;
+        col_len[tid] = n > cap ? kNoSlot : n;
+      }
+      __syncthreads();
+      uint32_t n = lane < R * 8 ? col_len[lane] : 0;
+      if (n == kNoSlot) n = 0;
+      len = __reduce_max_sync(0xffffffffu, n);
+      shortest = __reduce_min_sync(0xffffffffu, n ? n : kNoSlot);
+    }
+    const uint32_t tiles = (len + kTile - 1) / kTile;
+    const uint32_t mine_n = tiles > gw ? (tiles - gw + C * W - 1) / (C * W) : 0;  // this warp's tiles
     auto clear_columns = [&](uint32_t rows) {  // columns D.. of the tiles are zero (the join writes over them)
       const uint32_t extra = DP * (uint32_t)sizeof(T) / 16 - chunks;
       for (uint32_t e = lane; e < rows * extra; e += 32)
         *reinterpret_cast<uint4*>(ring + (e / extra) * A::kRow + (chunks + e % extra) * 16) = make_uint4(0, 0, 0, 0);
     };
     // The page number of position j, table entry `at`, and its row at slot `in` for the tile from j0 on.
-    auto page_at = [&](uint32_t j, uint32_t at) { return j < len && !too_long ? pages[at] : kNoSlot; };
+    auto page_at = [&](uint32_t j, uint32_t at) { return j < len ? pages[at] : kNoSlot; };
     auto row_of = [&](uint32_t p, uint32_t in, uint32_t j0) {
       if (p >= c.n_pages) {
-        bad |= j0 + ahead < len;
+        if (R == 1)
+          bad |= j0 + ahead < len;
+        else if (j0 + ahead < len)
+          first_bad = min(first_bad, j0 + ahead);
         return kNoSlot;
       }
       return (p * c.kvheads + h) * c.page + in;
@@ -516,44 +610,155 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
       copy_commit();
       j0 += step;
     }
-    q.split(r.scale * 1.4426950408889634f);
-    float o[DP / 16][4], m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
+    uint32_t len0[R], len1[R];
+    float undo0[R], undo1[R];
+    if constexpr (R == 1) {
+      q.split(r.scale * 1.4426950408889634f);
+      len0[0] = len1[0] = len;
+    } else {
+      for (uint32_t u = warp; u < units; u += W) {
+        const uint32_t x = x0 + u * 8 + g;
+        q.fetch(r.q + column(x < columns ? x : 0) * D, D, x < columns);
+        q.split(r.scale * 1.4426950408889634f);
 #pragma unroll
-    for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
+        for (int k = 0; k < A::kKS; k++)
+#pragma unroll
+          for (int p = 0; p < A::kQP; p++)
+            *reinterpret_cast<uint2*>(planes + ((u * A::kKS + k) * 32 + lane) * A::kQP * 2 + p * 2) =
+                make_uint2(q.f[k][p][0], q.f[k][p][1]);
+        if (t == 0) col_undo[u * 8 + g] = q.undo;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        len0[u] = col_len[u * 8 + 2 * t];
+        len1[u] = col_len[u * 8 + 2 * t + 1];
+        undo0[u] = __is_same(T, __half) && u < units ? col_undo[u * 8 + 2 * t] : 1.f;
+        undo1[u] = __is_same(T, __half) && u < units ? col_undo[u * 8 + 2 * t + 1] : 1.f;
+      }
+    }
+    float o[R][DP / 16][4], m0[R], m1[R], l0[R], l1[R];
+#pragma unroll
+    for (int u = 0; u < R; u++) {
+      m0[u] = m1[u] = -FLT_MAX;
+      l0[u] = l1[u] = 0.f;
+#pragma unroll
+      for (auto& x : o[u]) x[0] = x[1] = x[2] = x[3] = 0.f;
+    }
     for (uint32_t n = 0, slot = 0; n < mine_n; n++, slot = slot + 1 == NS ? 0 : slot + 1) {
       copy_wait<NS - 1>();
       __syncwarp();
-      const uint32_t tile_a = ring_a + slot * A::kStage;
-      float x[4];
-      q.scores(tile_a, x);
-      const uint32_t pos = gw * kTile + n * step + g;
-      if (pos >= len) x[0] = x[1] = -INFINITY;
-      if (pos + 8 >= len) x[2] = x[3] = -INFINITY;
-      const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
-      if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
-        float n0 = fmaxf(t0, m0), n1 = fmaxf(t1, m1);
+      const uint32_t tile_a = ring_a + slot * A::kStage, base = gw * kTile + n * step, pos = base + g;
+      float x[R][4];
+      if constexpr (R == 1) {
+        q.scores(tile_a, x[0]);
+      } else {
+        auto frag = [&](int u, int k, uint32_t (&b)[A::kQP][2]) {
 #pragma unroll
-        for (int w = 4; w < 32; w *= 2) {
-          n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
-          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
+          for (int p = 0; p < A::kQP; p++) {
+            const uint2 w = *reinterpret_cast<const uint2*>(planes + ((u * A::kKS + k) * 32 + lane) * A::kQP * 2 + p * 2);
+            b[p][0] = w.x;
+            b[p][1] = w.y;
+          }
+        };
+        if (units == R)
+          scores_of<T, DP, R, true>(tile_a, R, frag, x);
+        else
+          scores_of<T, DP, R, false>(tile_a, units, frag, x);
+#pragma unroll
+        for (int u = 0; u < R; u++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[u][e] *= e % 2 ? undo1[u] : undo0[u];
+      }
+      if (R == 1 || base + kTile > shortest) {
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+          if (pos >= len0[u]) x[u][0] = -INFINITY;
+          if (pos >= len1[u]) x[u][1] = -INFINITY;
+          if (pos + 8 >= len0[u]) x[u][2] = -INFINITY;
+          if (pos + 8 >= len1[u]) x[u][3] = -INFINITY;
         }
-        const float f0 = pow2(m0 - n0), f1 = pow2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= f0;
-        l1 *= f1;
+        if constexpr (R > 1) {
+          // Slots that one row attends to and another does not may hold anything for the latter: a row of V that
+          // is not finite becomes zeros, and the columns that attend to it NaN.
+          constexpr uint32_t kCh = DP * sizeof(T) / 16;
+          uint8_t* const v = ring + slot * A::kStage + kTile * A::kRow;
+          uint32_t wild = 0;
+          for (uint32_t e = lane; e < kTile * kCh; e += 32) {
+            const uint4 y = *reinterpret_cast<const uint4*>(v + (e / kCh) * A::kRow + e % kCh * 16);
+            bool any = false;
+            const uint32_t ws[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (auto& y : o) {
-          y[0] *= f0;
-          y[1] *= f1;
-          y[2] *= f0;
-          y[3] *= f1;
+            for (const uint32_t w : ws) {
+              constexpr uint32_t kExp = A::kF32 || !__is_same(T, __half) ? 0x7f800000u : 0x7c000000u;
+              any |= (w & kExp) == kExp || (!A::kF32 && (w & kExp >> 16) == kExp >> 16);
+            }
+            wild |= any ? 1u << e / kCh : 0u;
+          }
+          wild = __reduce_or_sync(0xffffffffu, wild);
+          if (wild) {
+            for (uint32_t e = lane; e < kTile * kCh; e += 32)
+              if (wild >> e / kCh & 1)
+                *reinterpret_cast<uint4*>(v + (e / kCh) * A::kRow + e % kCh * 16) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+            const uint32_t same_t = 0x11111111u << t;
+#pragma unroll
+            for (int u = 0; u < R; u++) {
+              const uint32_t b0 = __ballot_sync(0xffffffffu, (wild >> g & 1 && pos < len0[u]) || (wild >> (g + 8) & 1 && pos + 8 < len0[u]));
+              const uint32_t b1 = __ballot_sync(0xffffffffu, (wild >> g & 1 && pos < len1[u]) || (wild >> (g + 8) & 1 && pos + 8 < len1[u]));
+#pragma unroll
+              for (auto& y : o[u]) {
+                if (b0 & same_t) y[0] = y[2] = __int_as_float(0x7fc00000);
+                if (b1 & same_t) y[1] = y[3] = __int_as_float(0x7fc00000);
+              }
+            }
+          }
         }
       }
-      const float p[4] = {pow2(x[0] - m0), pow2(x[1] - m1), pow2(x[2] - m0), pow2(x[3] - m1)};
-      l0 += p[0] + p[2];
-      l1 += p[1] + p[3];
-      add_values<T, DP>(tile_a + kTile * A::kRow, p, o);
+      float t0[R], t1[R];
+      bool grows = false;
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        t0[u] = fmaxf(x[u][0], x[u][2]);
+        t1[u] = fmaxf(x[u][1], x[u][3]);
+        grows |= t0[u] > m0[u] || t1[u] > m1[u];
+      }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+          float n0 = fmaxf(t0[u], m0[u]), n1 = fmaxf(t1[u], m1[u]);
+#pragma unroll
+          for (int w = 4; w < 32; w *= 2) {
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
+          }
+          const float f0 = pow2(m0[u] - n0), f1 = pow2(m1[u] - n1);
+          m0[u] = n0;
+          m1[u] = n1;
+          l0[u] *= f0;
+          l1[u] *= f1;
+#pragma unroll
+          for (auto& y : o[u]) {
+            y[0] *= f0;
+            y[1] *= f1;
+            y[2] *= f0;
+            y[3] *= f1;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        x[u][0] = pow2(x[u][0] - m0[u]);
+        x[u][1] = pow2(x[u][1] - m1[u]);
+        x[u][2] = pow2(x[u][2] - m0[u]);
+        x[u][3] = pow2(x[u][3] - m1[u]);
+        l0[u] += x[u][0] + x[u][2];
+        l1[u] += x[u][1] + x[u][3];
+      }
+      if (R == 1 || units == R)
+        add_values<T, DP, R, true>(tile_a + kTile * A::kRow, R, x, o);
+      else
+        add_values<T, DP, R, false>(tile_a + kTile * A::kRow, units, x, o);
       __syncwarp();
       fetch(slot, row_of(next, next_in, j0), j0);
       copy_commit();
@@ -565,95 +770,113 @@ __global__ void __launch_bounds__(W * 32, Att<T, DP>::fixed(W) <= 75 * 1024 ? 3 
     copy_wait<0>();
     // the warps of the block: O and sums relative to the block's maxima, then added up
 #pragma unroll
-    for (int w = 4; w < 32; w *= 2) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, w);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, w);
-    }
-    if (g == 0) {
-      warp_m[warp * 8 + 2 * t] = m0;
-      warp_m[warp * 8 + 2 * t + 1] = m1;
-    }
-    bad = __syncthreads_or(bad) || too_long;
-    float M0 = m0, M1 = m1;
+    for (int u = 0; u < R; u++) {
 #pragma unroll
-    for (int w = 0; w < W; w++) {
-      M0 = fmaxf(M0, warp_m[w * 8 + 2 * t]);
-      M1 = fmaxf(M1, warp_m[w * 8 + 2 * t + 1]);
+      for (int w = 4; w < 32; w *= 2) {
+        l0[u] += __shfl_xor_sync(0xffffffffu, l0[u], w);
+        l1[u] += __shfl_xor_sync(0xffffffffu, l1[u], w);
+      }
+      if (g == 0) {
+        warp_m[(warp * R + u) * 8 + 2 * t] = m0[u];
+        warp_m[(warp * R + u) * 8 + 2 * t + 1] = m1[u];
+      }
     }
-    const float f0 = pow2(m0 - M0), f1 = pow2(m1 - M1);
-    float* const mine = reinterpret_cast<float*>(ring);  // [8][kO], sums
+    if constexpr (R == 1) {
+      bad = __syncthreads_or(bad);
+    } else {
+      first_bad = __reduce_min_sync(0xffffffffu, first_bad);
+      if (lane == 0) warp_bad[warp] = first_bad;
+      __syncthreads();
+      cluster_arrive();  // (q's planes are read, so in_o may be written)
+    }
+    float* const mine = reinterpret_cast<float*>(ring);  // [R][kPart]
 #pragma unroll
-    for (int m = 0; m < DP / 16; m++)
+    for (int u = 0; u < R; u++) {
+      float M0 = m0[u], M1 = m1[u];
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        mine[(2 * t + e % 2) * A::kO + m * 16 + g + (e / 2) * 8] = o[m][e] * (e % 2 ? f1 : f0);
-    if (g == 0) {
-      mine[8 * A::kO + 2 * t] = l0 * f0;
-      mine[8 * A::kO + 2 * t + 1] = l1 * f1;
+      for (int w = 0; w < W; w++) {
+        M0 = fmaxf(M0, warp_m[(w * R + u) * 8 + 2 * t]);
+        M1 = fmaxf(M1, warp_m[(w * R + u) * 8 + 2 * t + 1]);
+      }
+      const float f0 = pow2(m0[u] - M0), f1 = pow2(m1[u] - M1);
+      float* const part = mine + u * kPart;
+#pragma unroll
+      for (int m = 0; m < DP / 16; m++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          part[(2 * t + e % 2) * A::kO + m * 16 + g + (e / 2) * 8] = o[u][m][e] * (e % 2 ? f1 : f0);
+      if (g == 0) {
+        part[8 * A::kO + 2 * t] = l0[u] * f0;
+        part[8 * A::kO + 2 * t + 1] = l1[u] * f1;
+      }
     }
     __syncthreads();
     cluster_wait();  // the other blocks run, and have read what was sent for the previous turn
     // what they add up to goes to the blocks of the cluster: a share of O to each, maxima and sums to all
-    auto part = [&](uint32_t w) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage); };
+    auto part = [&](uint32_t w, uint32_t u) { return reinterpret_cast<const float*>(sm + w * NS * A::kStage) + u * kPart; };
     const uint32_t share = (2 * DP + C - 1) / C;  // 16-byte pieces of O of one block (the last may have fewer)
-    for (uint32_t e = tid; e < 2 * DP; e += W * 32) {
-      const uint32_t hh = e / (DP / 4), d = e % (DP / 4) * 4;
-      float4 sum = *reinterpret_cast<const float4*>(part(0) + hh * A::kO + d);
+    for (uint32_t ue = tid; ue < units * 2 * DP; ue += W * 32) {
+      const uint32_t u = ue / (2 * DP), e = ue % (2 * DP), hh = e / (DP / 4), d = e % (DP / 4) * 4;
+      float4 sum = *reinterpret_cast<const float4*>(part(0, u) + hh * A::kO + d);
 #pragma unroll
       for (int w = 1; w < W; w++) {
-        const float4 y = *reinterpret_cast<const float4*>(part(w) + hh * A::kO + d);
+        const float4 y = *reinterpret_cast<const float4*>(part(w, u) + hh * A::kO + d);
         sum.x += y.x;
         sum.y += y.y;
         sum.z += y.z;
         sum.w += y.w;
       }
       const uint32_t to = e / share;
-      st_cluster4(cluster_addr(smem_addr(in_o) + (rank * share + e - to * share) * 16, to), sum);
+      st_cluster4(cluster_addr(smem_addr(in_o) + ((u * C + rank) * share + e - to * share) * 16, to), sum);
     }
-    for (uint32_t e = tid; e < C * 8; e += W * 32) {
-      const uint32_t hh = e % 8, to = e / 8;
-      float M = warp_m[hh], L = part(0)[8 * A::kO + hh];
+    for (uint32_t e = tid; e < units * C * 8; e += W * 32) {
+      const uint32_t hh = e % 8, to = e / 8 % C, u = e / 8 / C;
+      float M = warp_m[u * 8 + hh], L = part(0, u)[8 * A::kO + hh];
 #pragma unroll
       for (int w = 1; w < W; w++) {
-        M = fmaxf(M, warp_m[w * 8 + hh]);
-        L += part(w)[8 * A::kO + hh];
+        M = fmaxf(M, warp_m[(w * R + u) * 8 + hh]);
+        L += part(w, u)[8 * A::kO + hh];
       }
-      const uint32_t a = cluster_addr(smem_addr(in_m) + rank * 16 * 4, to);
+      if constexpr (R > 1) {
+        const uint32_t n = col_len[u * 8 + hh];
+        bad = n == kNoSlot;
+#pragma unroll
+        for (int w = 0; w < W; w++) bad |= warp_bad[w] < n;
+      }
+      const uint32_t a = cluster_addr(smem_addr(in_m) + (u * kMaxCluster + rank) * 16 * 4, to);
       st_cluster(a + hh * 4, M);
       st_cluster(a + 32 + hh * 4, bad ? __int_as_float(0x7fc00000) : L);
     }
     cluster_sync();
-    // the maximum and the sum of head hh over the blocks (bad: NaN)
-    auto total = [&](uint32_t hh, float& M, float& L) {
-      M = -FLT_MAX;
-      L = 0.f;
+    for (uint32_t ue = tid; ue < units * share; ue += W * 32) {
+      const uint32_t u = ue / share, e = ue % share;
+      const uint32_t hh = (rank * share + e) / (DP / 4), d = (rank * share + e) % (DP / 4) * 4, x = x0 + u * 8 + hh;
+      if (hh >= 8 || x >= columns || d >= D) continue;  // (pieces behind the last belong to column 8)
+      const float* const ms = in_m + u * kMaxCluster * 16 + hh;
+      // the maximum and the sum of the column over the blocks (bad: NaN)
+      float M = -FLT_MAX, L = 0.f;
 #pragma unroll 4
-      for (uint32_t k = 0; k < C; k++) M = fmaxf(M, in_m[k * 16 + hh]);
+      for (uint32_t k = 0; k < C; k++) M = fmaxf(M, ms[k * 16]);
 #pragma unroll 4
-      for (uint32_t k = 0; k < C; k++) L = fmaf(in_m[k * 16 + 8 + hh], pow2(in_m[k * 16 + hh] - M), L);
-    };
-    const uint64_t row_head = (uint64_t)i * r.heads + h * G + g0;
-    for (uint32_t e = tid; e < share; e += W * 32) {
-      const uint32_t hh = (rank * share + e) / (DP / 4), d = (rank * share + e) % (DP / 4) * 4;
-      if (hh >= gn || d >= D) continue;  // (pieces behind the last belong to head 8)
-      float M, L;
-      total(hh, M, L);
+      for (uint32_t k = 0; k < C; k++) L = fmaf(ms[k * 16 + 8], pow2(ms[k * 16] - M), L);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (uint32_t k = 0; k < C; k++) {
-        const float f = pow2(in_m[k * 16 + hh] - M);
-        const float4 y = reinterpret_cast<const float4*>(in_o)[k * share + e];
+        const float f = pow2(ms[k * 16] - M);
+        const float4 y = reinterpret_cast<const float4*>(in_o)[(u * C + k) * share + e];
         sum.x = fmaf(y.x, f, sum.x);
         sum.y = fmaf(y.y, f, sum.y);
         sum.z = fmaf(y.z, f, sum.z);
         sum.w = fmaf(y.w, f, sum.w);
       }
+      if (R > 1 && col_len[u * 8 + hh] == 0) {  // (what it holds of the others' tiles means nothing)
+        sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        L = 0.f;
+      }
       const float inv = L == 0.f ? 0.f : (__is_same(T, __half) ? 1.f / 16384.f : 1.f) / L;
-      *reinterpret_cast<float4*>(r.out + (row_head + hh) * D + d) =
-          make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-      if (d == 0 && r.lse) r.lse[row_head + hh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+      *reinterpret_cast<float4*>(r.out + column(x) * D + d) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+      if (d == 0 && r.lse) r.lse[column(x)] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
-    if (g0 + 8 < G) cluster_arrive();
   }
 }
 
@@ -785,7 +1008,7 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32, 3) k_paged_weights(PagedK
         auto read = [&] {
           const uint32_t gn = min(8u, G - g0);
           const uint64_t head = (uint64_t)i * r.heads + h * G + g0;
-          q.fetch(r.q + head * D, D, gn);
+          q.fetch(r.q + (head + g) * D, D, g < gn);
           next0 = 2 * t < gn ? r.lse[head + 2 * t] : INFINITY;
           next1 = 2 * t + 1 < gn ? r.lse[head + 2 * t + 1] : INFINITY;
         };
@@ -1130,40 +1353,41 @@ cudaError_t launch_paged_append(const PagedKV& c, const float* k, const float* v
 namespace {
 
 
-template <class T, int DP, int W>
+template <class T, int DP, int W, int R>
 cudaError_t att_prepare() {
-  auto* f = k_paged_attention<T, DP, W>;
-  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, Att<T, DP>::fixed(W));
+  static_assert(Att<T, DP>::fixed(W, R) <= 227 * 1024, "shared memory of a block");
+  auto* f = k_paged_attention<T, DP, W, R>;
+  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, Att<T, DP>::fixed(W, R));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
 }
 
-// A cluster of C blocks of W warps a (row, KV head).
-template <class T, int DP, int W>
-cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, cudaStream_t st) {
+// A cluster of C blocks of W warps takes a row and KV head, or with R > 1 a group of `rows` rows.
+template <class T, int DP, int W, int R>
+cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_t rows, cudaStream_t st) {
   using A = Att<T, DP>;
-  static_assert(A::fixed(W) <= 227 * 1024, "shared memory of a block");
-  AttSplit sp{C, 0, 0, false};
+  AttSplit sp{C, 0, 0, rows, false};
+  const uint32_t clusters = R > 1 ? (r.rows + rows - 1) / rows : r.rows;
   // Where the blocks take two to three turns on the GPU, the short rows should be the last: 21 sequences of
   // 0..1531 positions in f32 29.5 -> 24.5 us, 64 of 130..4096 in bf16 60.5 -> 58.8, but 64 of 4096 each, where
   // it only delays the start, 100 -> 106; with more turns the end matters less than the start.
-  const uint32_t blocks = r.rows * c.kvheads * sp.blocks;
-  sp.longest_first = r.rows > 1 && r.rows <= kMaxSorted && blocks > 3 * 148 && blocks <= 8 * 148;
-  const uint32_t step = W * kTile * sp.blocks;
+  const uint32_t blocks = clusters * c.kvheads * C;
+  sp.longest_first = R == 1 && r.rows > 1 && r.rows <= kMaxSorted && blocks > 3 * 148 && blocks <= 8 * 148;
+  const uint32_t step = W * kTile * C;
   sp.step_pages = step / c.page;
   sp.step_slots = step % c.page;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(r.rows * sp.blocks, c.kvheads);
+  cfg.gridDim = dim3(clusters * C, c.kvheads);
   cfg.blockDim = dim3(W * 32);
-  cfg.dynamicSmemBytes = A::fixed(W);
+  cfg.dynamicSmemBytes = A::fixed(W, R);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = sp.blocks;
+  at[0].val.clusterDim.x = C;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, W>, c, r, sp);
+  return cudaLaunchKernelEx(&cfg, k_paged_attention<T, DP, W, R>, c, r, sp);
 }
 
 // Blocks of a cluster, and warps of a block.  Where the largest clusters leave SMs to spare, as many as there
@@ -1176,14 +1400,33 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, cudaStr
 template <class T, int DP>
 cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   using A = Att<T, DP>;
-  const uint32_t units = r.rows * c.kvheads, tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
-  uint32_t C = 1;
+  const uint32_t tiles = (uint32_t)(((uint64_t)c.max_pages * c.page + kTile - 1) / kTile);
+  cudaError_t e = cudaSuccess;
+  uint32_t C = 1, rows = 1;
+  if (r.shared) {
+    // Groups of neighbouring rows of one sequence, as prompts have them, read every tile once: as many rows as
+    // make R units of 8 columns.  512 rows of 4096 positions, 32/4 heads of 128 bf16: 449 us -> 361, 256 rows of
+    // 1024 with 8/8 heads of 64 f16 75 -> 19.  Other rows are left to the other kernel; where there are many, two
+    // kernels take longer than one (60 single rows beside a prompt's 100: 157 us against 120; 30 beside 256: 222
+    // against 211), so the callers ask for groups only where nearly all rows form them.
+    const uint32_t G = r.heads / c.kvheads;
+    rows = 8 * A::kShared / G;
+    if (rows < 2) rows = 1;
+    if (rows > 1) {
+      const uint32_t units = (r.rows + rows - 1) / rows * c.kvheads;
+      while (C < (uint32_t)kMaxCluster && tiles > A::W * C && units * C < 148) C *= 2;
+      e = att_launch<T, DP, A::W, A::kShared>(c, r, C, rows, st);
+      C = 1;
+    }
+  }
+  const uint32_t units = r.rows * c.kvheads;
   while (C < (uint32_t)kMaxCluster && tiles > A::W * C &&
          (units * C < 148 || (units * C < 700 && tiles >= 12 * A::W * C)))
     C *= 2;
   if (C == (uint32_t)kMaxCluster && units > 384 / C) C = 384 / units > 8 ? 384 / units : 8;
   const bool wide = units * C <= 148 && tiles > A::W * C;
-  cudaError_t e = wide ? att_launch<T, DP, A::kWide>(c, r, C, st) : att_launch<T, DP, A::W>(c, r, C, st);
+  if (e == cudaSuccess)
+    e = wide ? att_launch<T, DP, A::kWide, 1>(c, r, C, rows, st) : att_launch<T, DP, A::W, 1>(c, r, C, rows, st);
   if (r.weights && e == cudaSuccess) {
     using B = Give<T, DP>;
     const uint32_t smem = B::kSmem + c.n_seqs * 4, per_sm = 225 * 1024 / (smem + 1024);
@@ -1217,8 +1460,9 @@ struct AttPrepare {
   cudaError_t operator()() const {
     using A = Att<T, DP>;
     static_assert(Give<T, DP>::kSmem + (int)kMaxWeightSeqs * 4 <= 227 * 1024, "shared memory of a block");
-    cudaError_t e = att_prepare<T, DP, A::W>();
-    if (e == cudaSuccess) e = att_prepare<T, DP, A::kWide>();
+    cudaError_t e = att_prepare<T, DP, A::W, 1>();
+    if (e == cudaSuccess) e = att_prepare<T, DP, A::kWide, 1>();
+    if (e == cudaSuccess) e = att_prepare<T, DP, A::W, A::kShared>();
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(k_paged_weights<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                Give<T, DP>::kSmem + (int)kMaxWeightSeqs * 4);

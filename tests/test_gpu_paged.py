@@ -494,3 +494,73 @@ def test_calls_at_once_on_two_streams(cuda_engine, torch_cuda):
             c.handle(cuda_engine).attention(ptr(q), 32, 12, ptr(ln), ptr(o), stream=st.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(a, o) for a, o in zip(alone, outs))
+
+
+@pytest.mark.parametrize("kind,heads,kvheads,D,page", [
+    ("bf16", 32, 4, 128, 16),  # four rows share a sequence's tiles
+    ("f16", 4, 4, 64, 16),     # one head a KV head: 32 rows
+    ("f32", 6, 2, 96, 24),     # three: ten rows, 30 of 32 columns
+    ("f16", 10, 2, 72, 7),     # five: six rows; pages of single lookups
+    ("bf16", 34, 2, 32, 16),   # seventeen: one row, three parts of eight heads
+    ("f32", 64, 2, 128, 64),
+    ("bf16", 20, 1, 256, 16),  # twenty, two parts of eight at a time
+    ("f16", 32, 1, 192, 3),
+    ("f32", 2, 1, 256, 16),
+    ("f32", 9, 3, 4, 5),
+])
+def test_rows_of_prompts_share_tiles(cuda_engine, torch_cuda, kind, heads, kvheads, D, page):
+    """Many more rows than sequences: prompts' rows side by side, single rows between them, padding, rows of no
+    positions, all in one call."""
+    lens = [901, 64, 33, 0, 300]
+    cache = Cache(kind, kvheads, D, page, lens, seed=6, cap=950)
+    seq = [0] * 37 + [1] + [4] * 9 + [-1] * 2 + [2, 0, 2, 0] + [4] * 3 + [3] + [1] * 16 + [7] + [4] * 20
+    want = [901 - 37 + 1 + i for i in range(37)] + [64] + list(range(1, 10)) + [5, 5] + [33, 900, 1, 0]
+    want += [300, 0, 299] + [0] + list(range(49, 65)) + [3] + list(range(281, 301))
+    q = torch.randn(len(seq), heads, D, generator=torch.Generator().manual_seed(1)).cuda()
+    real = [i for i, s in enumerate(seq) if 0 <= s < 5]
+    before = torch.rand(5, kvheads, cache.cap, generator=torch.Generator().manual_seed(2)).cuda()
+    weights = before.clone()
+    out, lse = run_attention(cuda_engine, cache, q, seq, want, weights=weights)
+    check_attention(cache, q[real], [seq[i] for i in real], [want[i] for i in real], out[real], lse[real],
+                    weights=weights, before=before)
+    for i, s in enumerate(seq):
+        if not 0 <= s < 5:
+            assert bool((out[i] == 7).all()) and bool((lse[i] == 7).all())
+    again, _ = run_attention(cuda_engine, cache, q, seq, want)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_rows_that_share_tiles_do_not_share_what_is_wrong(cuda_engine, torch_cuda, kind):
+    """Infinities, NaN and invalid pages behind a row's length, and a neighbour longer than the cache, leave
+    the row as it is; rows that reach them are not finite."""
+    cache = Cache(kind, 2, 64, 16, [200, 150], seed=8)
+    q = torch.randn(32, 8, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    at = lambda s, j: (int(cache.table[s, j // 16]), slice(None), j % 16)
+    cache.v[at(0, 190)] = float("inf")
+    cache.v[at(0, 197)] = float("nan")
+    cache.k[at(0, 198)] = float("nan")
+    cache.table[1, 8] = cache.n_pages  # positions 128..143
+    seq, over = [0] * 16 + [1] * 16, cache.cap + 1
+    lens = [190, 191, 180, 200, 0, over, 190, 5, 199, 190, 100, 16, 0, 191, 198, 1]
+    lens += [128, 129, 150, 127, 1, 17, 0, over, 128, 128, 64, 150, 144, 100, 16, 127]
+    last = [190, 128]  # the longest that nothing is wrong with
+    good = [i for i in range(32) if lens[i] <= last[seq[i]]]
+    before = torch.rand(2, 2, cache.cap, generator=torch.Generator().manual_seed(2)).cuda()
+    weights = before.clone()
+    out, lse = run_attention(cuda_engine, cache, q, seq, lens, weights=weights)
+    check_attention(cache, q[good], [seq[i] for i in good], [lens[i] for i in good], out[good], lse[good])
+    for i in range(32):
+        if i not in good:
+            assert not bool(out[i].isfinite().any()), i
+    for i in [i for i in range(32) if lens[i] == over or (seq[i] and lens[i] > 128)]:
+        assert bool(out[i].isnan().all()) and bool(lse[i].isnan().all()), i
+    # rows that reach an infinite value still have weights (their scores are finite); the others' are exact
+    fine = [i for i in range(32) if i in good or (seq[i] == 0 and lens[i] <= 198)]
+    w = before.double()
+    _, _, ws, _, ew = attention64(cache, q[fine], [seq[i] for i in fine], [lens[i] for i in fine], 0.125)
+    bound = torch.zeros_like(w)
+    for i, x, e in zip(fine, ws, ew):
+        w[seq[i], :, :lens[i]] += x
+        bound[seq[i], :, :lens[i]] += e + 2.0 ** -23 * (w[seq[i], :, :lens[i]] + e)
+    assert bool(((weights.double() - w).abs() <= bound).all())
