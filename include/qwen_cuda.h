@@ -264,7 +264,8 @@ int qc_batch_ep_connect(qc_batch* b, const void* handles, const int* device_ids)
  * is checked there: a row of a sequence >= n_seqs (padding) is skipped and its outputs left as they
  * were; a length beyond max_pages * page or a page number >= n_pages among the slots a row uses makes
  * its results NaN (attention), or leaves the slot or the sequence as it was (append, evict).
- * Calls that write the same cache, weights or outputs must be ordered by the caller. */
+ * Calls that write the same cache, weights or outputs must be ordered by the caller; what a call writes
+ * lies apart from what it reads, where nothing else is said. */
 
 /* Row i of k and v ([rows][kvheads][head_dim] f32) goes, rounded to nearest, to slot pos[i] of sequence
  * seq[i] (seq NULL: sequence i).  The rows of a call have different slots.  weights (may be NULL, as for

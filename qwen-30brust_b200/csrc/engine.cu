@@ -1132,8 +1132,8 @@ struct qc_batch {
     pg->pool_bytes = (uint64_t)n_pages * c.kvheads * page * c.head_dim * (kind == qc::F32 ? 4 : 2);
     pg->table.assign(seqs * pg->per_seq, qc::kNoSlot);
     pg->cached.assign(n_seqs, 0);
-    for (uint32_t i = n_pages; i-- > 0;) pg->unused.push_back(i);
     QC_CK(cudaMalloc(&pg->d_pool, 2 * c.layers * pg->pool_bytes));
+    for (uint32_t i = n_pages; i-- > 0;) pg->unused.push_back(i);  // (a count that fits the device)
     QC_CK(cudaMalloc(&pg->d_table, pg->table.size() * 4));
     QC_CK(cudaMalloc(&pg->d_rows, 3ull * cap * 4));
     QC_CK(cudaMemsetAsync(pg->d_table, 0xff, pg->table.size() * 4, e->stream));
