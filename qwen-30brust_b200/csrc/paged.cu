@@ -889,9 +889,10 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
 // sequences that rows name and their longest rows in one pass over seq and len; their spans go to the warps
 // in turn.  Where there are fewer spans than warps these are shorter, and a row's q is read while the one
 // before is computed: 24 rows of 7001 positions, 4 KV heads, 44 -> 36 us for this pass; 128 rows of 1024, 16
-// query heads a KV head, 356 -> 155.  (Keeping the attention's scores in shared memory instead left one block an SM for long
-// sequences: 8 of 29,292..35,385 positions, 6 heads of 64 bf16, 113 us against 58 this way; 32 of
-// 200..2500, 32 heads of 128 f16, 39 against 41.)
+// query heads a KV head, 356 -> 155; 32 rows of 200..2500, 32/4 heads of 128 f16, whose spans stay whole, 43.3 ->
+// 45.5 with their attention.  (Keeping the attention's scores in shared memory instead left one block an SM for
+// long sequences: 8 of 29,292..35,385 positions, 6 heads of 64 bf16, 113 us against 58 this way; 32 of 200..2500
+// 39 against 41.)
 template <class T, int DP>
 struct Give {
   using A = Att<T, DP>;
