@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
 // in turn.  Where there are fewer spans than warps these are shorter, and a row's q is read while the one
 // before is computed: 24 rows of 7001 positions, 4 KV heads, 44 -> 36 us for this pass; 128 rows of 1024, 16
 // query heads a KV head, 356 -> 155; 32 rows of 200..2500, 32/4 heads of 128 f16, whose spans stay whole, 43.3 ->
-// 45.5 with their attention.  (Keeping the attention's scores in shared memory instead left one block an SM for
+// 44.2 with their attention.  (Keeping the attention's scores in shared memory instead left one block an SM for
 // long sequences: 8 of 29,292..35,385 positions, 6 heads of 64 bf16, 113 us against 58 this way; 32 of 200..2500
 // 39 against 41.)
 template <class T, int DP>
@@ -971,8 +971,6 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32, 3) k_paged_weights(PagedK
 #pragma unroll
         for (uint32_t u = 0; u < kTiles; u++) {
           constexpr uint32_t kCh = DP * sizeof(T) / 16;
-          old[u] = w0[u] = w8[u] = 0.f;
-          if (u >= tiles) continue;
 #pragma unroll 4
           for (uint32_t e = lane; e < kTile * kCh; e += 32) {
             const uint32_t pos = e / kCh, ch = e % kCh, src = __shfl_sync(0xffffffffu, row[u], pos);
@@ -982,7 +980,8 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32, 3) k_paged_weights(PagedK
                      src != kNoSlot);
           }
           const uint32_t slot = j0 + u * kTile + g + 8 * t;
-          if (t < 2 && slot < longest) old[u] = w[slot];
+          old[u] = t < 2 && u < tiles && slot < longest ? w[slot] : 0.f;
+          w0[u] = w8[u] = 0.f;
         }
         copy_commit();
         // the sequence's rows that reach the span, 8 heads at a time; while one is computed the next is read
@@ -1018,7 +1017,7 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32, 3) k_paged_weights(PagedK
         copy_wait<0>();
         __syncwarp();
         while (more) {
-          const uint32_t len = reach;
+          const uint32_t len = min(reach, j0 + span);
           const float lse0 = fabsf(next0) < INFINITY ? next0 * 1.4426950408889634f : INFINITY;  // (inf: no weights)
           const float lse1 = fabsf(next1) < INFINITY ? next1 * 1.4426950408889634f : INFINITY;
           q.split(r.scale * 1.4426950408889634f);
@@ -1027,7 +1026,7 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32, 3) k_paged_weights(PagedK
 #pragma unroll
           for (uint32_t u = 0; u < kTiles; u++) {
             const uint32_t j = j0 + u * kTile;
-            if (u >= tiles || j >= len) break;
+            if (j >= len) break;
             float x[4];
             q.scores(tile_a + u * B::kTileBytes, x);
             const bool in0 = j + g < len, in8 = j + g + 8 < len;
