@@ -38,12 +38,15 @@ struct ApiError : std::runtime_error {
   ApiError(int c, const std::string& m) : std::runtime_error(m), code(c) {}
 };
 
+// (a reported error is not left behind as the last one: the next launch's check would take it for its own)
 #define QC_CK(call)                                                                                        \
   do {                                                                                                     \
     cudaError_t e_ = (call);                                                                               \
-    if (e_ != cudaSuccess)                                                                                 \
+    if (e_ != cudaSuccess) {                                                                               \
+      (void)cudaGetLastError();                                                                            \
       throw ApiError(e_ == cudaErrorMemoryAllocation ? QC_ERR_NOMEM : QC_ERR_CUDA,                         \
                      std::string(#call) + ": " + cudaGetErrorString(e_));                                  \
+    }                                                                                                      \
   } while (0)
 
 void ensure(bool c, const std::string& m, int code = QC_ERR_INVALID) {
