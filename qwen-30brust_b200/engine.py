@@ -410,13 +410,14 @@ class Engine:
 
     def _adopt(self, handle) -> None:
         """A batch of this engine: destroyed with it if it is still there (when both are collected in one
-        garbage cycle, their finalizers run in any order)."""
-        self.__dict__.setdefault("_batches", set()).add(handle.value)
+        garbage cycle, their finalizers run in any order).  The handle is the batch's own object."""
+        self.__dict__.setdefault("_batches", {})[handle.value] = handle
 
     def close(self) -> None:
-        """Destroys the engine, and its batches first."""
-        for b in self.__dict__.pop("_batches", ()):
+        """Destroys the engine, and its batches first: their further calls raise QwenCudaError."""
+        for b in self.__dict__.pop("_batches", {}).values():
             lib().qc_batch_destroy(b)
+            b.value = None
         if getattr(self, "_h", None):
             lib().qc_engine_destroy(self._h)
             self._h = None
@@ -544,10 +545,8 @@ class Batch:
 
     def close(self) -> None:
         if getattr(self, "_h", None):
-            live = self.engine.__dict__.get("_batches", set())
-            if self._h.value in live:  # (else the engine has taken it along)
-                live.remove(self._h.value)
-                lib().qc_batch_destroy(self._h)
+            self.engine.__dict__.get("_batches", {}).pop(self._h.value, None)
+            lib().qc_batch_destroy(self._h)  # (null where the engine has taken it along)
             self._h = None
 
     def __del__(self):
