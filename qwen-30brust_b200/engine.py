@@ -473,7 +473,8 @@ class Batch:
         """qc_batch_logprobs of the sequences' latest logits: (log probabilities of ids [n][n_ids], entropies [n],
         the `top` likeliest ids [n][top], their log probabilities)."""
         sq = np.ascontiguousarray(seq_ids, dtype=np.uint32)
-        want = np.ascontiguousarray(ids if ids is not None else np.empty((sq.size, 0)), dtype=np.uint32).reshape(sq.size, -1)
+        want = np.ascontiguousarray(ids if ids is not None and sq.size else np.empty((sq.size, 0)), dtype=np.uint32)
+        want = want.reshape(sq.size, want.size // max(1, sq.size))
         out = _logprob_arrays(sq.size, want.shape[1], top)
         self._check(lib().qc_batch_logprobs(self._h, sq.ctypes.data, sq.size, want.ctypes.data, want.shape[1], top,
                                             *[a.ctypes.data for a in out]))

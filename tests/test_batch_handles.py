@@ -90,3 +90,23 @@ def test_an_engine_closed_under_its_batches(cuda_engine, tools):
             with pytest.raises(cuda_engine.QwenCudaError, match="null batch"):
                 call()
         b.close()
+
+
+def test_log_probabilities_of_no_sequence_are_refused(made):
+    """By the library, as every bad call (here the batch is gone as well)."""
+    E, _, eng, batches = made
+    eng.close()
+    for ids in (None, [], [[]], [[1, 2]]):
+        with pytest.raises(E.QwenCudaError):
+            batches[0].logprobs([], ids, 2)
+
+
+@pytest.mark.gpu
+def test_log_probabilities_of_no_sequence(cuda_engine, tools):
+    eng = cuda_engine.Engine(tools.synth_gguf(tools.TINY), 32)
+    b = cuda_engine.Batch(eng, 2, 32)
+    b.forward([0, 1], [1, 2])
+    for ids in (None, [], [[]]):
+        with pytest.raises(cuda_engine.QwenCudaError, match="empty batch"):
+            b.logprobs([], ids, 2)
+    assert b.logprobs([1, 0], [[3], [4]])[0].shape == (2, 1) and b.logprobs([1, 0], [3, 4])[0].shape == (2, 1)
