@@ -1,0 +1,88 @@
+"""Paged attention where keys or values are as large as their type allows.
+
+Bounds are attention64's: a slot without weight adds nothing to them."""
+import math
+
+import pytest
+import torch
+
+from _paged import DTYPE, Cache, attention64, ptr
+
+pytestmark = pytest.mark.gpu
+
+SHARED = [1, 32]  # rows of a sequence: by themselves, and together (16 rows a sequence and more)
+
+
+def run(E, cache, q, seq, lens, weights=None):
+    sq, ln = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (seq, lens))
+    out = torch.full(q.shape, 7.0, device="cuda")
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    cache.handle(E).attention(ptr(q), q.shape[1], len(lens), ptr(ln), ptr(out), seq_ptr=ptr(sq), lse_ptr=ptr(lse),
+                              weights_ptr=ptr(weights))
+    torch.cuda.synchronize()
+    return out, lse
+
+
+def put(cache, pool, s, j, value):
+    """value: of slot j of sequence s, all KV heads."""
+    getattr(cache, pool)[int(cache.table[s, j // cache.page]), :, j % cache.page] = value
+
+
+def without(cache, hidden):
+    """Sequence 0 without its first `hidden` slots, as a cache of its own."""
+    n = cache.lens[0] - hidden
+    rest = Cache(cache.kind, cache.kvheads, cache.D, cache.page, [n])
+    for pool in "kv":
+        rows = cache.rows(0, cache.lens[0], pool)[hidden:]
+        for j in range(n):
+            put(rest, pool, 0, j, rows[j])
+    return rest
+
+
+def check_hidden(E, cache, q, hidden, rows):
+    """The first `hidden` slots have no weight; a row that sees only them sees nothing."""
+    n = cache.lens[0]
+    seq, lens = [0] * rows, [n] * rows
+    if rows > 1:
+        lens[1], lens[rows - 1] = hidden, n - 1
+    weights = torch.zeros(1, cache.kvheads, cache.cap, device="cuda")
+    out, lse = run(E, cache, q, seq, lens, weights)
+    rest = without(cache, hidden)
+    seen = [i for i in range(rows) if lens[i] > hidden]
+    want, wlse, _, eo, _ = attention64(rest, q[seen], [0] * len(seen), [lens[i] - hidden for i in seen], 1 / math.sqrt(cache.D))
+    for k, i in enumerate(seen):
+        assert bool(((out[i].double() - want[k]).abs() <= eo[k]).all()), i
+        assert torch.allclose(lse[i].double(), wlse[k], rtol=2e-6, atol=2e-5), i
+    for i in set(range(rows)) - set(seen):
+        assert bool((out[i] == 0).all()) and bool((lse[i] == -math.inf).all())
+    assert bool((weights[..., :hidden] == 0).all()) and bool(weights[..., :n].isfinite().all())
+
+
+@pytest.mark.parametrize("rows", SHARED)
+@pytest.mark.parametrize("D,page", [(64, 16), (96, 5), (128, 16), (256, 24)])
+def test_f32_keys_of_the_lowest_value_have_no_weight(cuda_engine, torch_cuda, D, page, rows):
+    """-FLT_MAX and what rounds to it, against queries with zeros among their values."""
+    cache = Cache("f32", 2, D, page, [50], seed=D)
+    lowest = -torch.finfo(torch.float32).max
+    for j in range(7):
+        put(cache, "k", 0, j, lowest * (1 - j * 2.0 ** -14))
+    q = torch.full((rows, 8, D), 4.0, device="cuda")
+    q[:, :, 1::3] = 0
+    check_hidden(cuda_engine, cache, q, 7, rows)
+
+
+@pytest.mark.parametrize("rows", SHARED)
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,page", [(64, 16), (96, 5), (256, 24)])
+def test_values_of_the_largest_size(cuda_engine, torch_cuda, kind, D, page, rows):
+    cache = Cache(kind, 2, D, page, [50], seed=D)
+    most = torch.finfo(DTYPE[kind]).max
+    value = cache.rows(0, 50, "v")[3].clone()
+    value[:, 5], value[:, 6], value[:, 7] = most, -most, most * (1 - 2.0 ** -8)
+    put(cache, "v", 0, 3, value)
+    q = torch.randn(rows, 8, D, generator=torch.Generator().manual_seed(1)).cuda()
+    lens = [50 - i % 3 for i in range(rows)]
+    out, _ = run(cuda_engine, cache, q, [0] * rows, lens)
+    want, _, _, eo, _ = attention64(cache, q, [0] * rows, lens, 1 / math.sqrt(D))
+    for i in range(rows):
+        assert bool(out[i].isfinite().all()) and bool(((out[i].double() - want[i]).abs() <= eo[i]).all()), i
