@@ -278,8 +278,10 @@ int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_page
  * h / (heads / kvheads), at most 32 query heads per KV head.  out = softmax(scale q k^T) v in f32
  * (scale 0: 1 / sqrt(head_dim)); lse (may be NULL, [rows][heads]) receives log sum exp(scale q k^T).
  * A row of length 0 gives out 0 and lse -inf; so does one whose scores all overflow to -inf.  Slots a row
- * does not attend to may hold anything; a non-finite value among those it reads makes its results
- * non-finite.
+ * does not attend to may hold anything; a NaN or an infinite value among those it reads makes its results
+ * non-finite, but an infinite key counts as its score says (-inf: no weight).  The weighted values are added up
+ * before they are divided by the softmax's sum, relative to the largest weight: finite ones whose sum leaves
+ * f32's range give an infinity.
  * weights (may be NULL; needs lse, and n_seqs at most 8192): [n_seqs][kvheads][max_pages *
  * page] f32; the softmax weights that the rows give slot j, summed over a KV head's query heads, are added
  * to weights[s][kv head][j]; a head whose lse is NaN gives none.  The results do not depend on timing: the

@@ -168,7 +168,8 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
 }
 // x = hi + lo up to 2^-22 |x|, both with the 11 significant bits of tf32 (hi to nearest, ties away from zero; lo
 // cut).  What rounds beyond the largest such number is that number, so that finite values have finite parts; of an
-// infinity or a NaN lo keeps it.  In integers: 64 sequences of 130..4096 positions 137 us; with cvt.rna.tf32 143, bounded 151.
+// infinity or a NaN lo keeps it.  In integers: 64 sequences of 130..4096 positions 137 us; with
+// cvt.rna.tf32 143, and 151 with the bound.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   float h = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
   asm("min.xorsign.abs.f32 %0, %0, %1;" : "+f"(h) : "f"(__uint_as_float(0x7f7fe000u)));
@@ -276,10 +277,14 @@ __device__ __forceinline__ void scores_of(uint32_t ktile, uint32_t n, F&& frag, 
   for (int u = 0; u < R; u++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      if constexpr (A::kF32 || A::kQP == 3)
-        s[u][i] = c[u][0][i] + (c[u][1][i] + c[u][2][i]);
-      else
-        s[u][i] = c[u][0][i] + c[u][1][i];
+      // An infinite sum of the first planes is the score: the other planes' may be infinite the other way (keys of
+      // the type's lowest value, queries rounded up) or NaN (infinite keys, queries without a second plane).  f32
+      // keys that are NaN are so in their second plane.
+      const float first = c[u][0][i];
+      float rest = c[u][1][i];
+      if constexpr (A::kF32 || A::kQP == 3) rest += c[u][2][i];
+      const bool all = fabsf(first) == INFINITY && (!A::kF32 || c[u][A::kF32 ? 2 : 0][i] == c[u][A::kF32 ? 2 : 0][i]);
+      s[u][i] = all ? first : first + rest;
     }
 }
 
@@ -321,6 +326,8 @@ struct Query {
         const float x = raw[k][0] * factor, y = raw[k][1] * factor;
         split_tf32(x, f[k][0][0], f[k][1][0]);
         split_tf32(y, f[k][0][1], f[k][1][1]);
+        if (x != x) f[k][0][0] = 0x7fffe000u;  // (NaN in the first plane too)
+        if (y != y) f[k][0][1] = 0x7fffe000u;
       }
     } else {
       float up = 1.f;
