@@ -1290,8 +1290,9 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(PagedKV c, PagedEv
 // Rows kept[i] of K or V to slot i, in 16-byte pieces: block (x: sequence and KV head; y:
 // K or V, and its share of a row's pieces; z: its share of the rows).  In place a sequence's rows move to
 // lower slots, kept[i] >= i ascending, so one block takes them all, tile by tile: a tile is written only
-// when the block has read it, and what it writes lies below all that later tiles read.  Elsewhere the tiles
-// are spread over the blocks.
+// when the block has read it, and what it writes lies below all that later tiles read.  The rows before the first
+// that moves are left alone, up to a 256th of all (64 sequences of 4000 slots of 4 x 128 bf16 within their budget:
+// 15 us, 400 with their rows written where they are).  Elsewhere the tiles are spread over the blocks.
 constexpr uint32_t kMoveThreads = 256, kMoveRows = 128;  // rows of a tile
 
 template <class T>
@@ -1310,8 +1311,12 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(PagedKV c, PagedEvi
   uint8_t* const pool = static_cast<uint8_t*>(blockIdx.y & 1 ? c.v : c.k) + c0 * 16;
   constexpr uint32_t kHold = 8;  // pieces a thread holds at once
   const uint32_t step_row = kMoveThreads / cn, step_piece = kMoveThreads % cn;
-  uint32_t turn = 0;
-  for (uint32_t r0 = blockIdx.z * kMoveRows; r0 < m; r0 += gridDim.z * kMoveRows, turn ^= 1) {
+  uint32_t turn = 0, r0 = blockIdx.z * kMoveRows;
+  if (e.dst_table == c.table) {  // (kept[i] - i never falls: who has it 0 at the end of a run has it 0 all through)
+    const uint32_t run = (m + kMoveThreads - 1) / kMoveThreads, last = min(m, (tid + 1) * run) - 1;
+    r0 = run * __syncthreads_count(tid * run < m && kept[last] == last);
+  }
+  for (; r0 < m; r0 += gridDim.z * kMoveRows, turn ^= 1) {
     const uint32_t rows = min(kMoveRows, m - r0);
     if (tid < rows) {
       from_row[turn][tid] = (uint32_t)pool_row(c, c.table, s, h, kept[r0 + tid]);
