@@ -259,8 +259,8 @@ int qc_batch_ep_connect(qc_batch* b, const void* handles, const int* device_ids)
  * All arguments that are not sizes are DEVICE pointers on one device (pools, q, k, v and out 16-byte
  * aligned); the call runs on that device and on `stream` (a cudaStream_t of that device; NULL = its
  * default stream), allocates nothing, keeps nothing between calls and returns once the work is
- * enqueued, so it can be captured into a CUDA graph (the first call on a device loads the kernels: make
- * it before a capture).  Errors: qc_last_error().  What lies on the device
+ * enqueued, so it can be captured into a CUDA graph (the first paged call, and the first qc_logprobs, on a
+ * device load their kernels: make them before a capture).  Errors: qc_last_error().  What lies on the device
  * is checked there: a row of a sequence >= n_seqs (padding) is skipped and its outputs left as they
  * were; a length beyond max_pages * page or a page number >= n_pages among the slots a row uses makes
  * its results NaN (attention), or leaves the slot or the sequence as it was (append, evict).

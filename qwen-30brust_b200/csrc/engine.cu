@@ -68,8 +68,17 @@ void prepare_device(int device) {
   QC_CK(qc::sample_prepare());
   QC_CK(qc::batch_prepare(kMaxSmem));
   QC_CK(qc::qgemm_prepare());
-  QC_CK(qc::paged_prepare());
   QC_CK(qc::logprobs_prepare());
+  done[device] = true;
+}
+// The same for the paged cache's kernels, three types by six widths of each: 24 ms, beside 10 for all others, that
+// only their users pay.
+void prepare_paged(int device) {
+  static std::mutex mu;
+  static bool done[64] = {};
+  std::lock_guard<std::mutex> lock(mu);
+  if (device < 0 || device >= 64 || done[device]) return;
+  QC_CK(qc::paged_prepare());
   done[device] = true;
 }
 
@@ -1308,6 +1317,7 @@ struct qc_batch {
            "and at most 32 query heads per KV head");
     QC_CK(cudaSetDevice(e->device));
     if (kind != qc::kNoSlot) {
+      prepare_paged(e->device);
       create_pages(kind, page, n_pages, weights);
     } else {
       kv_floats = (uint64_t)c.kvheads * ctx * D;
@@ -2374,10 +2384,10 @@ struct DevicePointers {
     if (device < 0) device = at.device;
     ensure(at.device == device, std::string(name) + " lives on another device than the other arguments");
   }
-  void enter() {
+  void enter(void (*prepare)(int)) {
     QC_CK(cudaGetDevice(&before));
     if (before != device) QC_CK(cudaSetDevice(device));
-    prepare_device(device);
+    prepare(device);
   }
 };
 
@@ -2416,7 +2426,7 @@ int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_page
     at.add(seq, "seq");
     at.add(pos, "pos");
     at.add(weights, "weights");
-    at.enter();
+    at.enter(prepare_paged);
     QC_CK(qc::launch_paged_append(c, k, v, rows, seq, pos, weights, static_cast<cudaStream_t>(stream)));
   });
 }
@@ -2447,7 +2457,7 @@ int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, 
     at.add(out, "out", 16);
     at.add(lse, "lse");
     at.add(weights, "weights");
-    at.enter();
+    at.enter(prepare_paged);
     qc::PagedRows r{q, heads, rows, seq, len, scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale, out, lse, weights,
                     rows / 16 >= n_seqs};
     QC_CK(qc::launch_paged_attention(c, r, static_cast<cudaStream_t>(stream)));
@@ -2473,7 +2483,7 @@ int qc_paged_evict(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_pages
     at.add(len, "len");
     at.add(new_len, "new_len");
     at.add(kept, "kept");
-    at.enter();
+    at.enter(prepare_paged);
     qc::PagedEvict e{weights, len, keep, recent, dst_table ? dst_table : table, kept, new_len, weights_out};
     QC_CK(qc::launch_paged_evict(c, e, static_cast<cudaStream_t>(stream)));
   });
@@ -2494,7 +2504,7 @@ int qc_logprobs(const float* logits, uint32_t rows, uint32_t n, uint64_t stride,
     at.add(entropy, "entropy");
     at.add(top_ids, "top_ids");
     at.add(top_logprobs, "top_logprobs");
-    at.enter();
+    at.enter(prepare_device);
     qc::LogprobArgs a{logits, nullptr, rows, n, stride, ids, n_ids, top, logprobs, entropy, top_ids, top_logprobs};
     QC_CK(qc::launch_logprobs(a, static_cast<cudaStream_t>(stream)));
   });
