@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __
 //   O^T [D x 8 heads]           += V^T P^T        (V read transposed; P^T by an 8x8 register transpose)
 // The operands keep f32 accuracy: q and p are split into planes of the page type whose sum is exact to
 // 2^-22 (f16: two, scaled by a power of two to stay in range) or 2^-24 (bf16: three); f32 pages are
-// split themselves, into two tf32 planes.  A tile's products are added to f32 sums outside the matrix
+// split themselves, into two tf32 planes (2^-22), and the product of the two smaller parts is left out (2^-24 to
+// 2^-22 of the product; adding it changed no error).  A tile's products are added to f32 sums outside the matrix
 // units, whose accumulators truncate.  Queries of one KV head share K and V; more than 8 heads take
 // another turn over the sequence, 8 at a time.
 //
@@ -237,12 +238,18 @@ __device__ __forceinline__ float pow2(float x) {
 // for position lane / 4 and columns 2 (lane % 4), + 1; s[u][2], s[u][3] for position lane / 4 + 8.  frag(u, k, b):
 // the planes of q^T of unit u, step k.  All: n = R; without a test at every unit the compiler interleaves their
 // products (512 rows of 4096 positions, 32/4 heads of 128 bf16: 361 us against 489).
-template <class T, int DP, int R, bool All, class F>
+//
+// The matrix units cut their sums at every step, D / 8 of them in f32: there hi x hi goes to H sums in turn and the
+// smaller products to L others.  Four and one where rows are computed by themselves: errors of 3e-7 to 6e-7 of the
+// outputs, about the plain form's or below it, where one and two give 5e-7 to 1.4e-6 in the same time.  Two and one
+// for R units, whose registers hold no more (64 rows of 2048 positions 83 us, with three and one 93), two and two
+// for the weights (with one 188 us for those rows, against 181).
+template <class T, int DP, int R, bool All, int H, int L, class F>
 __device__ __forceinline__ void scores_of(uint32_t ktile, uint32_t n, F&& frag, float (&s)[R][4]) {
   using A = Att<T, DP>;
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t a0 = ktile + ((lane / 8 % 2) * 8 + lane % 8) * A::kRow + (lane / 16) * 16;
-  float c[R][A::kF32 ? 3 : A::kQP][4];
+  float c[R][A::kF32 ? H + L : A::kQP][4];
 #pragma unroll
   for (auto& u : c)
 #pragma unroll
@@ -259,9 +266,9 @@ __device__ __forceinline__ void scores_of(uint32_t ktile, uint32_t n, F&& frag, 
       for (int u = 0; u < R; u++) {
         if (!All && u >= n) break;
         frag(u, k, b);
-        mma8(c[u][0], hi, b[0][0], b[0][1]);
-        mma8(c[u][1], hi, b[1][0], b[1][1]);
-        mma8(c[u][2], lo, b[0][0], b[0][1]);
+        mma8(c[u][k % H], hi, b[0][0], b[0][1]);
+        mma8(c[u][H], hi, b[1][0], b[1][1]);
+        mma8(c[u][H + L - 1], lo, b[0][0], b[0][1]);
       }
     } else {
 #pragma unroll
@@ -277,14 +284,18 @@ __device__ __forceinline__ void scores_of(uint32_t ktile, uint32_t n, F&& frag, 
   for (int u = 0; u < R; u++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      // An infinite sum of the first planes is the score: the other planes' may be infinite the other way (keys of
-      // the type's lowest value, queries rounded up) or NaN (infinite keys, queries without a second plane).  f32
-      // keys that are NaN are so in their second plane.
-      const float first = c[u][0][i];
-      float rest = c[u][1][i];
-      if constexpr (A::kF32 || A::kQP == 3) rest += c[u][2][i];
-      const bool all = fabsf(first) == INFINITY && (!A::kF32 || c[u][A::kF32 ? 2 : 0][i] == c[u][A::kF32 ? 2 : 0][i]);
-      s[u][i] = all ? first : first + rest;
+      float first = c[u][0][i];
+      if constexpr (A::kF32) {
+#pragma unroll
+        for (int p = 1; p < H; p++) first += c[u][p][i];
+        s[u][i] = first + (L == 2 ? c[u][H][i] + c[u][H + L - 1][i] : c[u][H][i]);
+      } else {
+        // An infinite sum of the first planes is the score: the other planes' may be infinite the other way (keys
+        // of the type's lowest value, queries rounded up) or NaN (infinite keys, queries without a second plane).
+        float rest = c[u][1][i];
+        if constexpr (A::kQP == 3) rest += c[u][2][i];
+        s[u][i] = fabsf(first) == INFINITY ? first : first + rest;
+      }
     }
 }
 
@@ -293,6 +304,7 @@ __device__ __forceinline__ void scores_of(uint32_t ktile, uint32_t n, F&& frag, 
 template <class T, int DP>
 struct Query {
   using A = Att<T, DP>;
+  static constexpr bool kScaled = A::kF32 || __is_same(T, __half);
   float raw[A::kKS][A::kF32 ? 2 : 4];
   uint32_t f[A::kKS][A::kQP][2];
   float undo0, undo1, undo;  // (undo: of column lane / 4)
@@ -320,32 +332,32 @@ struct Query {
   __device__ __forceinline__ void split(float factor) {
     const uint32_t t = threadIdx.x & 3;
     undo0 = undo1 = undo = 1.f;
+    float up = 1.f;
+    if constexpr (kScaled) {
+      // the largest |q| of a head: f16, to 2^13..2^14, so that two planes hold 22 bits; f32, to 2^-10..2^-9, so that
+      // no sum of the parts' products overflows before the score does
+      constexpr int kTo = A::kF32 ? -10 : 13;
+      float mx = 0.f;
+#pragma unroll
+      for (int k = 0; k < A::kKS; k++)
+#pragma unroll
+        for (int b = 0; b < (A::kF32 ? 2 : 4); b++) mx = fmaxf(mx, fabsf(raw[k][b] * factor));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      int e = kTo - ((int)(__float_as_uint(mx) >> 23) - 127);
+      e = mx == 0.f || mx > FLT_MAX ? 0 : e > 120 ? 120 : e < -126 ? -126 : e;
+      up = __uint_as_float((uint32_t)(127 + e) << 23);
+      undo = __uint_as_float((uint32_t)(127 - e) << 23);
+      undo0 = __shfl_sync(0xffffffffu, undo, 8 * t);
+      undo1 = __shfl_sync(0xffffffffu, undo, 8 * t + 4);
+    }
     if constexpr (A::kF32) {
 #pragma unroll
       for (int k = 0; k < A::kKS; k++) {
-        const float x = raw[k][0] * factor, y = raw[k][1] * factor;
-        split_tf32(x, f[k][0][0], f[k][1][0]);
-        split_tf32(y, f[k][0][1], f[k][1][1]);
-        if (x != x) f[k][0][0] = 0x7fffe000u;  // (NaN in the first plane too)
-        if (y != y) f[k][0][1] = 0x7fffe000u;
+        split_tf32(raw[k][0] * factor * up, f[k][0][0], f[k][1][0]);
+        split_tf32(raw[k][1] * factor * up, f[k][0][1], f[k][1][1]);
       }
     } else {
-      float up = 1.f;
-      if constexpr (__is_same(T, __half)) {  // the largest |q| of a head to 2^13..2^14: two planes hold 22 bits
-        float mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < A::kKS; k++)
-#pragma unroll
-          for (int b = 0; b < 4; b++) mx = fmaxf(mx, fabsf(raw[k][b] * factor));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
-        e = mx == 0.f || mx > FLT_MAX ? 0 : e > 120 ? 120 : e;
-        up = __uint_as_float((uint32_t)(127 + e) << 23);
-        undo = __uint_as_float((uint32_t)(127 - e) << 23);
-        undo0 = __shfl_sync(0xffffffffu, undo, 8 * t);
-        undo1 = __shfl_sync(0xffffffffu, undo, 8 * t + 4);
-      }
 #pragma unroll
       for (int k = 0; k < A::kKS; k++) {
         const float x[4] = {raw[k][0] * factor * up, raw[k][1] * factor * up, raw[k][2] * factor * up,
@@ -362,9 +374,10 @@ struct Query {
     }
   }
 
+  template <int H, int L>
   __device__ __forceinline__ void scores(uint32_t ktile, float (&s)[4]) const {
     float x[1][4];
-    scores_of<T, DP, 1, true>(ktile, 1, [&](int, int k, uint32_t (&b)[A::kQP][2]) {
+    scores_of<T, DP, 1, true, H, L>(ktile, 1, [&](int, int k, uint32_t (&b)[A::kQP][2]) {
 #pragma unroll
       for (int p = 0; p < A::kQP; p++) {
         b[p][0] = f[k][p][0];
@@ -644,8 +657,8 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
       for (int u = 0; u < R; u++) {
         len0[u] = col_len[u * 8 + 2 * t];
         len1[u] = col_len[u * 8 + 2 * t + 1];
-        undo0[u] = __is_same(T, __half) && u < units ? col_undo[u * 8 + 2 * t] : 1.f;
-        undo1[u] = __is_same(T, __half) && u < units ? col_undo[u * 8 + 2 * t + 1] : 1.f;
+        undo0[u] = Query<T, DP>::kScaled && u < units ? col_undo[u * 8 + 2 * t] : 1.f;
+        undo1[u] = Query<T, DP>::kScaled && u < units ? col_undo[u * 8 + 2 * t + 1] : 1.f;
       }
     }
     float o[R][DP / 16][4], m0[R], m1[R], l0[R], l1[R];
@@ -662,7 +675,7 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
       const uint32_t tile_a = ring_a + slot * A::kStage, base = gw * kTile + n * step, pos = base + g;
       float x[R][4];
       if constexpr (R == 1) {
-        q.scores(tile_a, x[0]);
+        q.template scores<4, 1>(tile_a, x[0]);
       } else {
         auto frag = [&](int u, int k, uint32_t (&b)[A::kQP][2]) {
 #pragma unroll
@@ -673,9 +686,9 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
           }
         };
         if (units == R)
-          scores_of<T, DP, R, true>(tile_a, R, frag, x);
+          scores_of<T, DP, R, true, 2, 1>(tile_a, R, frag, x);
         else
-          scores_of<T, DP, R, false>(tile_a, units, frag, x);
+          scores_of<T, DP, R, false, 2, 1>(tile_a, units, frag, x);
 #pragma unroll
         for (int u = 0; u < R; u++)
 #pragma unroll
@@ -1043,7 +1056,7 @@ __global__ void __launch_bounds__(Give<T, DP>::W * 32, Give<T, DP>::kBlocks) k_p
             const uint32_t j = j0 + u * kTile;
             if (j >= len) break;
             float x[4];
-            q.scores(tile_a + u * B::kTileBytes, x);
+            q.template scores<2, 2>(tile_a + u * B::kTileBytes, x);
             const bool in0 = j + g < len, in8 = j + g + 8 < len;
             w0[u] += in0 && lse0 < INFINITY ? pow2(x[0] - lse0) : 0.f;
             w8[u] += in8 && lse0 < INFINITY ? pow2(x[2] - lse0) : 0.f;

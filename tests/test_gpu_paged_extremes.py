@@ -167,3 +167,28 @@ def test_nan_is_never_lost(cuda_engine, torch_cuda, kind, bits, rows):
     out, lse = run(cuda_engine, cache, q, [0] * rows, [50] * rows)
     assert not bool(out[:, 2].isfinite().any()) and not bool(lse[:, 2].isfinite().any())
     assert bool(out[:, [0, 1, 3, 4, 5, 6, 7]].isfinite().all())
+
+
+@pytest.mark.parametrize("rows", SHARED)
+@pytest.mark.parametrize("D", [96, 128, 192, 256])
+def test_f32_scores_are_not_cut_in_one_long_sum(cuda_engine, torch_cuda, D, rows):
+    """Products of one sign, whose sum the matrix units cut towards zero at every step of eight: the sum so far and
+    the step's eight products each by half a last place on average, at most 2^-24 of the sum.  m equal steps lose
+    m + 1 of those of their whole sum; rows by themselves have four sums of D / 32 steps, rows together two of D / 16.
+    lse is s + log n here, with s far larger; its own roundings, and those of queries and keys, are to the nearest and
+    vanish in the mean: 1.5 for what is left."""
+    n, heads = 100, 8
+    cache = Cache("f32", 2, D, 16, [n], seed=D)
+    g = torch.Generator().manual_seed(D)
+    for j in range(n):
+        put(cache, "k", 0, j, (0.5 + torch.rand(2, D, generator=g)).cuda())
+    q = 16 * (0.5 + torch.rand(rows if rows > 1 else 24, heads, D, generator=g)).cuda()
+    if rows > 1:
+        _, lse = run(cuda_engine, cache, q, [0] * rows, [n] * rows)
+    else:
+        lse = torch.cat([run(cuda_engine, cache, q[i:i + 1].contiguous(), [0], [n])[1] for i in range(24)])
+    _, want, _, _, _ = attention64(cache, q, [0] * len(q), [n] * len(q), 1 / math.sqrt(D))
+    want = torch.stack(want)
+    bias = float(((lse.double() - want) / want).mean()) / 2.0 ** -24
+    steps = D / (32 if rows == 1 else 16)
+    assert abs(bias) <= steps + 1 + 1.5, bias
