@@ -209,7 +209,8 @@ int qc_batch_logits_device(const qc_batch* b, uint32_t seq, const float** out);
 int qc_batch_sample(qc_batch* b, qc_sampler* const* samplers, const uint32_t* seq_ids, uint32_t n, uint32_t* tokens_out);
 /* The chat loop (main.rs:261-282) for n distinct sequences at once, on the device: `steps` times,
  * sample every sequence's latest logits with its sampler and run the n ids as one step.
- * tokens_out (host, may be NULL): steps x n ids, step-major. */
+ * tokens_out (host, may be NULL): steps x n ids, step-major.  A paged batch must have free pages for all steps
+ * beforehand, and evicts nothing between them. */
 int qc_batch_decode_sample(qc_batch* b, qc_sampler* const* samplers, const uint32_t* seq_ids, uint32_t n, uint32_t steps,
                            uint32_t* tokens_out);
 /* As qc_batch_create, with the sequences' caches in pages (see "paged key-value cache" below) instead of one
@@ -275,8 +276,9 @@ int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_page
                     const float* v, uint32_t rows, const uint32_t* seq, const uint32_t* pos, float* weights, void* stream);
 /* Attention of new tokens (ops.rs:57-98 over a paged cache): row i of q ([rows][heads][head_dim] f32)
  * attends to slots 0..len[i]-1 of sequence seq[i] (seq NULL: sequence i); head h reads KV head
- * h / (heads / kvheads), at most 32 query heads per KV head.  out = softmax(scale q k^T) v in f32
- * (scale 0: 1 / sqrt(head_dim)); lse (may be NULL, [rows][heads]) receives log sum exp(scale q k^T).
+ * h / (heads / kvheads), at most 32 query heads per KV head.  out = softmax(scale q k^T) v with f32 sums
+ * (scale 0: 1 / sqrt(head_dim); queries and softmax weights keep 22 bits beside f16 pages, 24 beside bf16, and f32
+ * pages' values 22 in the products, exponentials 22: the result is about as exact as f32 arithmetic); lse (may be NULL, [rows][heads]) receives log sum exp(scale q k^T).
  * A row of length 0 gives out 0 and lse -inf; so does one whose scores all overflow to -inf.  Slots a row
  * does not attend to may hold anything; a NaN or an infinite value among those it reads makes its results
  * non-finite, but an infinite key counts as its score says (-inf: no weight).  The weighted values are added up
@@ -284,8 +286,10 @@ int qc_paged_append(uint32_t kind, void* k_pages, void* v_pages, uint32_t n_page
  * f32's range give an infinity.
  * weights (may be NULL; needs lse, and n_seqs at most 8192): [n_seqs][kvheads][max_pages *
  * page] f32; the softmax weights that the rows give slot j, summed over a KV head's query heads, are added
- * to weights[s][kv head][j]; a head whose lse is NaN gives none.  The results do not depend on timing: the
- * same call gives the same bits. */
+ * to weights[s][kv head][j]; a head whose lse is not finite gives none.  They are exp(score - lse) with the f32 lse,
+ * off by about 2^-22 |lse| of themselves.  The results do not depend on timing: the same call gives the same bits.
+ * (Rows of one sequence side by side are computed together, which is quicker for prompts, where rows >= 16 n_seqs;
+ * a prompt in a table of many sequences is best given as a call with its own line of the table.) */
 int qc_paged_attention(uint32_t kind, const void* k_pages, const void* v_pages, uint32_t n_pages, uint32_t page,
                        uint32_t kvheads, uint32_t head_dim, const uint32_t* table, uint32_t n_seqs, uint32_t max_pages,
                        const float* q, uint32_t heads, uint32_t rows, const uint32_t* seq, const uint32_t* len, float scale,

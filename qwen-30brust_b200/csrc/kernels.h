@@ -315,7 +315,7 @@ struct PagedRows {
   float scale;
   float *out, *lse;  // [rows][heads][D], [rows][heads] or null
   float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights (needs lse)
-  bool shared;       // nearly all neighbouring rows are of one sequence
+  bool shared;       // neighbouring rows are expected to be of one sequence, nearly all (right either way)
 };
 constexpr uint32_t kMaxWeightSeqs = 8192;  // sequences of a call with weights
 constexpr uint32_t kNoSlot = 0xffffffffu;

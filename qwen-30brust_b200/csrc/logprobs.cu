@@ -14,7 +14,9 @@
 // the warps' has k values at or above it; it is taken after the first chunk, and again after the second
 // and the eighth.  A warp whose room for candidates runs out selects its k best and goes by them.  The
 // warps' parts are joined in shared memory, the blocks' parts and k best through distributed shared
-// memory.  No workspace, no atomics; the sums' order is fixed, and the candidates' keys differ.
+// memory.  No workspace, no atomics on global memory; the sums' order is fixed.  (Candidates are listed and ranked with
+// atomics in shared memory: their keys differ, so their order does not depend on it.)  VEC = 4 spills 44 bytes a
+// thread to hold four blocks an SM.
 #include <float.h>
 
 #include "kernels.h"
@@ -484,7 +486,7 @@ cudaError_t logprobs_prepare() {
 
 // Blocks a row: up to two an SM over all rows, of two chunks a warp at least.  (A block's start and end, its
 // thresholds and the exchange, take as long as several chunks: 128 rows of 151,936 values with 5
-// alternatives take 27 us with 2 blocks a row, 31 with 4, 40 with 8.)
+// alternatives take 28 us with 2 blocks a row, 31 with 4, 40 with 8.)
 cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st) {
   uint32_t logc = 0;
   while (logc < 4 && ((uint64_t)a.rows << (logc + 1)) <= 296 && a.n > (kLpWarps * 1024u) << logc) logc++;

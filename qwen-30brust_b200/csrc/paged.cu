@@ -50,8 +50,8 @@ __device__ __forceinline__ uint4 round16(const float* x) {
 
 // Row i's k and v (f32, rounded to nearest) to slot pos[i] of sequence seq[i]; its weights become 0.  A block
 // takes a row, a thread 16 bytes of the cache at a time, of k and of v.  A step's rows are bound by latency (the
-// row's place, then its values, then the write): 64 rows of 4 x 128 bf16 take 1.9 us; a prompt's by bytes:
-// 4500 rows of 8 x 128 f16 take 11.8 us, 4.7 TB/s.
+// row's place, then its values, then the write): 64 rows of 4 x 128 bf16 take 2.1 us; a prompt's by bytes:
+// 4500 rows of 8 x 128 f16 take 12.1 us, 4.6 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __restrict__ k, const float* __restrict__ v,
                                                        const uint32_t* __restrict__ seq, const uint32_t* __restrict__ pos,
@@ -90,8 +90,9 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedKV c, const float* __
 //
 // Neighbouring rows of one sequence (prompts) are taken R units of 8 (row, head) columns at a time, their q's
 // planes in shared memory: K and V come from L2 once for up to 8 R columns, and a unit's products fill the waits
-// of another's.  512 rows of 4096 positions, 32/4 heads of 128 bf16: 361 us, the matrix units busy about half
-// the time (48 products a tile and unit); a row at a time 449.
+// of another's.  512 rows of 4096 positions, 32/4 heads of 128 bf16: 362 us, the matrix units busy about half
+// the time (48 products a tile and unit); a row at a time 466.  These kernels use all 255 registers, and spill 8 to
+// 44 bytes a thread at most widths.
 //
 // The warps' (maximum, sum, O) are joined in shared memory, the blocks' through the cluster's
 // distributed shared memory in a fixed order: no workspace, no atomics, the same bits every time.
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
   }
   // Where pages hold whole runs of 8 positions a lane copies its part of a run with one address; else every
   // position has its own page and its lanes ask the lane that looked it up.  64 sequences of 4096
-  // positions in bf16: 100 us with pages of 16 slots (runs), 105 with pages of 250.
+  // positions in bf16: 105 us with pages of 16 slots (runs), 108 with pages of 250.
   const bool runs = c.page % 8 == 0;
   const uint32_t step = C * W * kTile, gw = rank * W + warp;
   const uint32_t ahead = runs ? lane / 16 * 8 : lane % kTile;  // the position of a tile this lane looks up
@@ -905,7 +906,8 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
 }
 
 // ---- accumulated weights -------------------------------------------------------------------------
-// The rows' softmax weights exp(s - lse), summed over a KV head's heads and a sequence's rows, added to the
+// The rows' softmax weights exp(s - lse) (lse is an f32 number, so that they are off by about 2^-22 |lse| of
+// themselves), summed over a KV head's heads and a sequence's rows, added to the
 // slots: a second pass over K with the lse that the attention has left, so that every slot is added to
 // once, whatever rows share a sequence, and the attention need not hold its scores.  A warp takes kTiles
 // tiles of 16 positions of a (sequence, KV head) at a time and goes through the sequence's rows in call
@@ -916,7 +918,7 @@ __global__ void __launch_bounds__(W * 32, R > 1 ? 2 : Att<T, DP>::fixed(W, R) <=
 // query heads a KV head, 356 -> 155; 32 rows of 200..2500, 32/4 heads of 128 f16, whose spans stay whole, 43.3 ->
 // 44.2 with their attention.  (Keeping the attention's scores in shared memory instead left one block an SM for
 // long sequences: 8 of 29,292..35,385 positions, 6 heads of 64 bf16, 113 us against 58 this way; 32 of 200..2500
-// 39 against 41.)
+// 39 against 41.)  Width 256 spills 104 (f16) to 640 bytes (f32) a thread, f32 220 at 192.
 template <class T, int DP>
 struct Give {
   using A = Att<T, DP>;
@@ -1401,9 +1403,10 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_
   using A = Att<T, DP>;
   AttSplit sp{C, 0, 0, rows, false};
   const uint32_t clusters = R > 1 ? (r.rows + rows - 1) / rows : r.rows;
-  // Where the blocks take two to three turns on the GPU, the short rows should be the last: 21 sequences of
-  // 0..1531 positions in f32 29.5 -> 24.5 us, 64 of 130..4096 in bf16 60.5 -> 58.8, but 64 of 4096 each, where
-  // it only delays the start, 100 -> 106; with more turns the end matters less than the start.
+  // Where the blocks take more than one turn on the GPU (three an SM) and fewer than three, the short rows should be
+  // the last: 21 sequences of 0..1531 positions in f32 26.9 -> 24.1 us, 64 of 130..4096 in bf16 63.1 -> 60.2, 96 of
+  // them 88.5 -> 84.6.  The lengths are not known here: equal ones lose by the later start (64 of 4096, 103 -> 106;
+  // 32 of them 62.6 -> 64.9).  With more turns the end matters less (128 of 130..2048: 62.5 either way).
   const uint32_t blocks = clusters * c.kvheads * C;
   sp.longest_first = R == 1 && r.rows > 1 && r.rows <= kMaxSorted && blocks > 3 * 148 && blocks <= 8 * 148;
   const uint32_t step = W * kTile * C;
@@ -1425,11 +1428,13 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_
 
 // Blocks of a cluster, and warps of a block.  Where the largest clusters leave SMs to spare, as many as there
 // are tiles for, and wide blocks (one sequence of 32,768 positions in bf16, 4 KV heads: 41.7 us with 4 warps,
-// 26 with 8).  Else enough small blocks to fill the GPU (three an SM) nearly twice, as the sequences' lengths
-// differ and are not known here, as long as a warp keeps six tiles of a full cache; 24 rows of 7001 positions
-// take 106 us with 8 blocks (768 in all), 118 with 6, 136 with 16.  Large clusters leave parts of a GPC
-// unused; where they would not all find room at once, clusters that do are better (32 units of 9000..32768
-// positions: 73 us with 12 blocks, 80 with 16, 88 with 8).
+// 26.5 with 8; of 8192, 14.2 and 12.0).  Else enough small blocks to fill the GPU (three an SM) nearly twice, as the
+// sequences' lengths differ and are not known here, as long as a warp keeps six tiles of a full cache: 64 of
+// 130..4096, 4 KV heads, 80 us with 1 block, 60 with this rule's 4, 75 with 8; 16 of 1000..8192, 46 with 4, 43 with
+// 8, 49 with 16.  Large clusters leave parts of a GPC unused; where they would not all find room at once, clusters
+// that do are better (8 of 9000..32768: 74 us with 12 blocks, 80 with 16, 87 with 8).
+// What the rule misses: equal lengths need no second turn (64 of 4096: 106 us, 90 with 1 block), and next to its
+// bounds half the blocks can be better (32 of 130..4096: 41 with 8, 36 with 4; 6 rows of 7001: 36 with 16, 23 with 8).
 template <class T, int DP>
 cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   using A = Att<T, DP>;
@@ -1438,10 +1443,14 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
   uint32_t C = 1, rows = 1;
   if (r.shared) {
     // Groups of neighbouring rows of one sequence, as prompts have them, read every tile once: as many rows as
-    // make R units of 8 columns.  512 rows of 4096 positions, 32/4 heads of 128 bf16: 449 us -> 361, 256 rows of
-    // 1024 with 8/8 heads of 64 f16 75 -> 19.  Other rows are left to the other kernel; where there are many, two
-    // kernels take longer than one (60 single rows beside a prompt's 100: 157 us against 120; 30 beside 256: 222
-    // against 211), so the callers ask for groups only where nearly all rows form them.
+    // make R units of 8 columns.  512 rows of 4096 positions, 32/4 heads of 128 bf16: 466 us -> 361, 256 rows of
+    // 1024 with 8/8 heads of 64 f16 75 -> 18.5; 8 rows of 4096, which fill fewer blocks, 17 -> 23.  Other rows are left
+    // to the other kernel.  Where there are many, two kernels take longer than one (60 single rows beside a prompt's
+    // 100: 157 us against 120; 30 beside 256: 222 against 211), so the callers ask for groups only where they expect
+    // nearly all rows to form them: a batch, which knows its rows, where 15 of 16 neighbours are of one sequence,
+    // qc_paged_attention where there are 16 rows for every sequence of the table.  That says nothing about the order:
+    // 512 rows of 4 sequences in turn form no group and take 464 us, 455 without the first launch, and 512 rows of one
+    // sequence in a table of 64 stay by themselves, 490 us instead of 372.
     const uint32_t G = r.heads / c.kvheads;
     rows = 8 * A::kShared / G;
     if (rows < 2) rows = 1;
