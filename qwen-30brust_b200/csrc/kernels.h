@@ -317,6 +317,7 @@ struct PagedRows {
   float* weights;    // [n_seqs][kvheads][max_pages * page] or null: += the rows' weights (needs lse)
   bool shared;       // neighbouring rows are expected to be of one sequence, nearly all (right either way)
 };
+constexpr uint32_t kSMs = 148;             // of the GPU that the launch rules of paged.cu and logprobs.cu are measured on
 constexpr uint32_t kMaxWeightSeqs = 8192;  // sequences of a call with weights
 constexpr uint32_t kNoSlot = 0xffffffffu;
 struct PagedEvict {

@@ -489,7 +489,7 @@ cudaError_t logprobs_prepare() {
 // alternatives take 28 us with 2 blocks a row, 31 with 4, 40 with 8.)
 cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st) {
   uint32_t logc = 0;
-  while (logc < 4 && ((uint64_t)a.rows << (logc + 1)) <= 296 && a.n > (kLpWarps * 1024u) << logc) logc++;
+  while (logc < 4 && ((uint64_t)a.rows << (logc + 1)) <= 2 * kSMs && a.n > (kLpWarps * 1024u) << logc) logc++;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.rows << logc);
   cfg.blockDim = dim3(kLpThreads);

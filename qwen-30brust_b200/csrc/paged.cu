@@ -1408,7 +1408,7 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, uint32_t C, uint32_
   // them 88.5 -> 84.6.  The lengths are not known here: equal ones lose by the later start (64 of 4096, 103 -> 106;
   // 32 of them 62.6 -> 64.9).  With more turns the end matters less (128 of 130..2048: 62.5 either way).
   const uint32_t blocks = clusters * c.kvheads * C;
-  sp.longest_first = R == 1 && r.rows > 1 && r.rows <= kMaxSorted && blocks > 3 * 148 && blocks <= 8 * 148;
+  sp.longest_first = R == 1 && r.rows > 1 && r.rows <= kMaxSorted && blocks > 3 * kSMs && blocks <= 8 * kSMs;
   const uint32_t step = W * kTile * C;
   sp.step_pages = step / c.page;
   sp.step_slots = step % c.page;
@@ -1456,23 +1456,23 @@ cudaError_t att_launch(const PagedKV& c, const PagedRows& r, cudaStream_t st) {
     if (rows < 2) rows = 1;
     if (rows > 1) {
       const uint32_t units = (r.rows + rows - 1) / rows * c.kvheads;
-      while (C < (uint32_t)kMaxCluster && tiles > A::W * C && units * C < 148) C *= 2;
+      while (C < (uint32_t)kMaxCluster && tiles > A::W * C && units * C < kSMs) C *= 2;
       e = att_launch<T, DP, A::W, A::kShared>(c, r, C, rows, st);
       C = 1;
     }
   }
   const uint32_t units = r.rows * c.kvheads;
   while (C < (uint32_t)kMaxCluster && tiles > A::W * C &&
-         (units * C < 148 || (units * C < 700 && tiles >= 12 * A::W * C)))
+         (units * C < kSMs || (units * C < 700 && tiles >= 12 * A::W * C)))
     C *= 2;
   if (C == (uint32_t)kMaxCluster && units > 384 / C) C = 384 / units > 8 ? 384 / units : 8;
-  const bool wide = units * C <= 148 && tiles > A::W * C;
+  const bool wide = units * C <= kSMs && tiles > A::W * C;
   if (e == cudaSuccess)
     e = wide ? att_launch<T, DP, A::kWide, 1>(c, r, C, rows, st) : att_launch<T, DP, A::W, 1>(c, r, C, rows, st);
   if (r.weights && e == cudaSuccess) {
     using B = Give<T, DP>;
     const uint32_t smem = B::kSmem + c.n_seqs * 4, per_sm = 225 * 1024 / (smem + 1024), most = B::kBlocks;
-    k_paged_weights<T, DP><<<148 * (per_sm > most ? most : per_sm), B::W * 32, smem, st>>>(c, r);
+    k_paged_weights<T, DP><<<kSMs * (per_sm > most ? most : per_sm), B::W * 32, smem, st>>>(c, r);
     e = cudaGetLastError();
   }
   return e;
@@ -1544,7 +1544,7 @@ cudaError_t launch_paged_evict(const PagedKV& c, const PagedEvict& e, cudaStream
   // blocks a sequence and KV head: to fill the GPU, of 4096 slots at least
   const uint32_t cap = c.max_pages * c.page;
   uint32_t logc = 0;
-  while (1u << logc < kSelBlocks && ((uint64_t)units << logc) < 148 && cap > 4096u << logc) logc++;
+  while (1u << logc < kSelBlocks && ((uint64_t)units << logc) < kSMs && cap > 4096u << logc) logc++;
   const uint32_t per = (cap + (1u << logc) - 1) >> logc, hold = per < kSelHold ? per : kSelHold;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(units << logc);
@@ -1563,9 +1563,9 @@ cudaError_t launch_paged_evict(const PagedKV& c, const PagedEvict& e, cudaStream
   // (64 bytes at least).
   uint32_t shares = 1, tiles = 1;
   if (e.dst_table == c.table)
-    while ((uint64_t)units * 2 * shares < 1184 && pieces / (shares * 2) >= 4) shares *= 2;
+    while ((uint64_t)units * 2 * shares < 8 * kSMs && pieces / (shares * 2) >= 4) shares *= 2;
   else
-    while ((uint64_t)units * 2 * tiles < 2368 && tiles * kMoveRows < e.keep) tiles *= 2;
+    while ((uint64_t)units * 2 * tiles < 16 * kSMs && tiles * kMoveRows < e.keep) tiles *= 2;
   QC_BY_KIND(c.kind, (k_evict_move<T><<<dim3(units, 2 * shares, tiles), kMoveThreads, 0, st>>>(c, e, shares)));
   return cudaGetLastError();
 }
